@@ -11,17 +11,6 @@ python -c "import __graft_entry__ as g; g.smoke()" | tail -1
 timeout 200 python bench.py --steps 12 --warmup 3 | tail -1
 timeout 200 python bench.py --model qwen3-30b-a3b --steps 12 --warmup 3 | tail -1
 
-# 1. XCD-granular StaggerU (the r02 per-WG variant broke GROUP_M L2
-#    sharing — profiles/README.md; the refinement staggers per L2
-#    domain only). A/B once implemented:
-TD_GEMM_STAGGER=1 timeout 240 python scripts/bench_stagger.py || true
-
-# 2. GEMM rate attack per the hipBLASLt SK3 ISA study
-#    (profiles/hipblaslt_sk3_isa_study.md): prototype the 4-wave
-#    128x128-per-wave tile with one direct-to-VGPR operand; numerics
-#    gate first, then the ladder:
-#    timeout 300 python scripts/bench_stream.py   # shape sweep harness
-
 # 3. If >1 physical GPU is ever available: burn-in FIRST
 #    (docs/ROADMAP.md item 1) — the spin overlap paths have never run
 #    on real xGMI peers:
