@@ -11,6 +11,8 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -35,34 +37,54 @@ def _needs_build(so: Path, srcs: list[Path]) -> bool:
     return any(p.stat().st_mtime > so_mtime for p in deps)
 
 
-def build(force: bool = False, verbose: bool = True) -> Path:
+def _hipcc() -> str:
+    return os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+
+
+def compile_command(src: Path, obj: Path) -> list[str]:
     import pybind11
 
-    srcs = _sources()
-    so = _so_path()
-    if not force and not _needs_build(so, srcs):
-        return so
-    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    py_include = sysconfig.get_paths()["include"]
-    cmd = [
-        hipcc,
+    return [
+        _hipcc(),
         f"--offload-arch={ARCH}",
         "-O3",
         "-std=c++17",
         "-fPIC",
-        "-shared",
         "-fvisibility=hidden",
         "-Wno-unused-result",
+        # packed fp32 instructions stay out: some of their forms are not
+        # reliable on this hardware
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         f"-I{CSRC / 'include'}",
-        f"-I{py_include}",
+        f"-I{sysconfig.get_paths()['include']}",
         f"-I{pybind11.get_include()}",
-        *[str(s) for s in srcs],
-        "-o",
-        str(so),
+        "-c", str(src), "-o", str(obj),
     ]
-    if verbose:
-        print("[triton_dist_amd.build]", " ".join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
+
+
+def link_command(objs: list[Path], so: Path) -> list[str]:
+    return [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC",
+            *[str(o) for o in objs], "-o", str(so)]
+
+
+def build(force: bool = False, verbose: bool = True) -> Path:
+    srcs = _sources()
+    so = _so_path()
+    if not force and not _needs_build(so, srcs):
+        return so
+    with tempfile.TemporaryDirectory() as tmp:
+        def one(src: Path) -> Path:
+            obj = Path(tmp) / (src.stem + ".o")
+            cmd = compile_command(src, obj)
+            if verbose:
+                print("[triton_dist_amd.build]", " ".join(cmd),
+                      file=sys.stderr)
+            subprocess.run(cmd, check=True)
+            return obj
+
+        with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+            objs = list(pool.map(one, srcs))
+        subprocess.run(link_command(objs, so), check=True)
     return so
 
 
