@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "td/api.hpp"
+#include "td/paged.hpp"
 
 namespace py = pybind11;
 using namespace td;
@@ -473,6 +474,95 @@ static void flash_decode_paged(uintptr_t q, uintptr_t kp, uintptr_t vp,
                             block, (void *)out, (const void *)off, batch,
                             qh, kvh, as_stream(stream));
   TD_CHECK_HIP(hipGetLastError());
+}
+
+// Operators over a paged cache: the cache comes as one list of 20 integers,
+// in the order in which ops/paged.py puts them.
+static PagedArgs paged_args(const std::vector<long> &c) {
+  if (c.size() != 20) throw std::runtime_error("paged cache: 20 fields");
+  PagedArgs a{};
+  a.k = (void *)c[0];
+  a.v = (void *)c[1];
+  a.k_page = c[2], a.k_row = c[3], a.k_head = c[4];
+  a.v_page = c[5], a.v_row = c[6], a.v_head = c[7];
+  a.n_blocks = c[8];
+  a.block = (int)c[9], a.kvh = (int)c[10], a.d = (int)c[11];
+  a.is_fp16 = (int)c[12];
+  a.table = {(const void *)c[13], (int)c[14]};
+  a.table_stride = c[15];
+  a.max_blocks = (int)c[16];
+  a.lens = {(const void *)c[17], (int)c[18]};
+  a.batch = (int)c[19];
+  return a;
+}
+
+static void paged_append(const std::vector<long> &cache, uintptr_t k,
+                         long k_tok, long k_head, uintptr_t v, long v_tok,
+                         long v_head, long tokens, uintptr_t cu, int cu64,
+                         uintptr_t key_pos, uintptr_t pos, int pos64,
+                         uintptr_t stream) {
+  launch_paged_append(paged_args(cache), (const void *)k, k_tok, k_head,
+                      (const void *)v, v_tok, v_head, tokens,
+                      {(const void *)cu, cu64}, (int *)key_pos,
+                      {(const void *)pos, pos64}, as_stream(stream));
+}
+
+static void paged_decode(const std::vector<long> &cache, uintptr_t q,
+                         long q_tok, long q_head, int qh, float scale,
+                         float softcap, uintptr_t slopes, uintptr_t key_pos,
+                         uintptr_t q_pos, int q_pos64, uintptr_t out,
+                         uintptr_t lse, uintptr_t mass, uintptr_t mass_out,
+                         uintptr_t ws, uintptr_t stream) {
+  PagedDecodeArgs a{};
+  a.c = paged_args(cache);
+  a.s = {scale, softcap, (const float *)slopes};
+  a.q = (const void *)q, a.q_tok = q_tok, a.q_head = q_head, a.qh = qh;
+  a.key_pos = (const int *)key_pos;
+  a.q_pos = {(const void *)q_pos, q_pos64};
+  a.out = (void *)out, a.lse = (float *)lse;
+  a.mass = (const float *)mass, a.mass_out = (float *)mass_out;
+  a.ws = (void *)ws;
+  launch_paged_decode(a, as_stream(stream));
+}
+
+static void kv_evict(const std::vector<long> &cache, uintptr_t mass,
+                     uintptr_t key_pos, int budget, int recent,
+                     uintptr_t mass_out, uintptr_t key_pos_out,
+                     uintptr_t lens_out, uintptr_t ws, uintptr_t stream) {
+  EvictArgs a{};
+  a.c = paged_args(cache);
+  a.mass = (const float *)mass, a.key_pos = (const int *)key_pos;
+  a.budget = budget, a.recent = recent;
+  a.mass_out = (float *)mass_out, a.key_pos_out = (int *)key_pos_out;
+  a.lens_out = (void *)lens_out;
+  a.ws = (void *)ws;
+  launch_kv_evict(a, as_stream(stream));
+}
+
+static void packed_prefill(uintptr_t q, long q_tok, long q_head, uintptr_t k,
+                           long k_tok, long k_head, uintptr_t v, long v_tok,
+                           long v_head, uintptr_t out, long out_tok,
+                           long out_head, uintptr_t lse, long rows, long keys,
+                           int qh, int kvh, int d, int is_fp16, int seqs,
+                           uintptr_t cu_q, int cu_q64, uintptr_t cu_k,
+                           int cu_k64, uintptr_t prefix, int prefix64,
+                           int causal, int clear_tail, float scale,
+                           float softcap, uintptr_t slopes,
+                           uintptr_t stream) {
+  PackedArgs a{};
+  a.q = (const void *)q, a.k = (const void *)k, a.v = (const void *)v;
+  a.q_tok = q_tok, a.q_head = q_head, a.k_tok = k_tok, a.k_head = k_head;
+  a.v_tok = v_tok, a.v_head = v_head;
+  a.out = (void *)out, a.out_tok = out_tok, a.out_head = out_head;
+  a.lse = (float *)lse;
+  a.rows = rows, a.keys = keys;
+  a.qh = qh, a.kvh = kvh, a.d = d, a.is_fp16 = is_fp16, a.seqs = seqs;
+  a.cu_q = {(const void *)cu_q, cu_q64};
+  a.cu_k = {(const void *)cu_k, cu_k64};
+  a.prefix = {(const void *)prefix, prefix64};
+  a.causal = causal, a.clear_tail = clear_tail;
+  a.s = {scale, softcap, (const float *)slopes};
+  launch_packed_prefill(a, as_stream(stream));
 }
 
 static void gdn_decode(uintptr_t q, uintptr_t k, uintptr_t v, uintptr_t g,
@@ -977,6 +1067,12 @@ PYBIND11_MODULE(_C, m) {
   m.def("reduce_scatter", &reduce_scatter_op);
   m.def("gdn_decode", &gdn_decode);
   m.def("flash_decode_paged", &flash_decode_paged);
+  m.def("paged_append", &paged_append);
+  m.def("paged_decode_workspace", &paged_decode_workspace);
+  m.def("paged_decode", &paged_decode);
+  m.def("kv_evict_workspace", &kv_evict_workspace);
+  m.def("kv_evict", &kv_evict);
+  m.def("packed_prefill", &packed_prefill);
   m.def("flash_prefill", &flash_prefill, py::arg("q"), py::arg("k"),
         py::arg("v"), py::arg("out"), py::arg("b"), py::arg("s"),
         py::arg("qh"), py::arg("kvh"), py::arg("scale"), py::arg("causal"),

@@ -77,3 +77,9 @@ from .gdn import (  # noqa: F401
     chunk_gated_delta_rule_fwd,
     gdn_decode_step,
 )
+from .paged import (  # noqa: F401
+    paged_append_op,
+    paged_decode_op,
+    kv_evict_op,
+    flash_prefill_packed_op,
+)
