@@ -67,108 +67,410 @@ __global__ __launch_bounds__(256) void k_paged_append(
 }
 
 // ---------------------------------------------------------------------------
-// decode: a workgroup per sequence and query head, a thread per key for the
-// scores, a thread per element of the output for the sums.
+// decode
+//
+// Bound by reading K and V once. The batch's keys are cut into chunks of
+// equal length on the device, from the lengths as they are, so a long
+// sequence among short ones is spread over the card as well; a workgroup
+// takes one chunk of one key head and up to 16 of its query heads.
+//
+// In a workgroup each of the four waves goes through 32-key tiles of its
+// own, without a barrier. S^T = K Q^T and O^T = V^T P^T, so that a lane
+// holds the scores of one query head all the way: lane (n, qd) = (lane & 15,
+// lane >> 4) gets from the 16x16x32 matrix instructions the scores of head n
+// and keys 16 t + 4 qd + i, which are the elements that the second product
+// wants from it, once its 32 keys are numbered (qd, t, i). K goes from
+// global memory to the operand's registers; V takes a way through the
+// wave's piece of LDS, where it is read transposed.
+//
+// The weights meet V in the inputs' type, as a rounded part and the rounded
+// rest: the second product is far from bounding the kernel, and with it the
+// output's own rounding is the only one that counts.
 // ---------------------------------------------------------------------------
-template <typename T>
-TD_DEV float score(const PagedDecodeArgs &a, const float *q, int b, int h,
-                   int slot, int len, long page) {
-  const int kh = h / (a.qh / a.c.kvh);
-  const T *row = (const T *)a.c.k + page * a.c.k_page +
-                 (slot % a.c.block) * a.c.k_row + kh * a.c.k_head;
-  float s = 0.f;
-  for (int i = 0; i < a.c.d; ++i) s += q[i] * (float)row[i];
-  s *= a.s.scale;
-  if (a.s.softcap > 0.f) s = a.s.softcap * tanhf(s / a.s.softcap);
-  if (a.s.slopes) {
-    long far = a.key_pos ? a.q_pos[b] - a.key_pos[((long)b * a.c.kvh + kh) *
-                                                      a.c.room() + slot]
-                         : (long)len - 1 - slot;
-    s -= a.s.slopes[h] * (float)(far < 0 ? -far : far);
-  }
-  return s;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kTile = 32;              // keys of a wave's step
+constexpr int kStep = 4 * kTile;       // keys of a workgroup's step
+constexpr int kSlots = 768;            // workgroups that the card holds
+
+template <typename T> using vec8 = __attribute__((ext_vector_type(8))) T;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+
+TD_DEV f32x4 mfma16(vec8<bf16> a, vec8<bf16> b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+TD_DEV f32x4 mfma16(vec8<_Float16> a, vec8<_Float16> b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// Of each 16 lanes, lane l gets column l of the 4x16 block whose row l / 4
+// and columns 4 (l % 4) on its pointer names.
+TD_DEV s16x4 read_transposed(const void *lds) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4 *)(unsigned)(uintptr_t)lds);
+}
+// Orders a wave's own LDS traffic for the compiler; the hardware keeps it
+// in order.
+TD_DEV void wave_fence() {
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_paged_decode(PagedDecodeArgs a) {
-  __shared__ float q[256], p[256], red[4], part[256];
-  const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const int d = a.c.d, kh = h / (a.qh / a.c.kvh);
-  const int len = a.c.len(b);
-  if (tid < d) q[tid] = (float)((const T *)a.q)[b * a.q_tok + h * a.q_head +
-                                                tid];
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  const int col = tid % d, lane = tid / d, lanes = 256 / d;
-  for (int base = 0; base < len; base += 256) {
-    __syncthreads();
-    const int slot = base + tid;
-    float s = -INFINITY;
-    if (slot < len) {
-      const long page = a.c.page(b, slot);
-      if (page >= 0) s = score<T>(a, q, b, h, slot, len, page);
+struct Chunk {
+  int b, len;        // sequence and its length
+  int first, count;  // this chunk's number among the sequence's, how many
+  int id;            // over the whole batch
+  int steps;         // of kStep keys, a chunk's length
+};
+
+// The chunk `id` of the batch, or (id < 0) sequence `seq`'s first one. A
+// sequence has one chunk at least. Every wave finds its own.
+TD_DEV bool find_chunk(const PagedArgs &c, int target, int least, int id,
+                       int seq, Chunk &out) {
+  const int lane = threadIdx.x & 63;
+  long total = 0;
+  int len = 0;
+  for (int base = 0; base < c.batch; base += 64) {
+    len = base + lane < c.batch ? c.len(base + lane) : 0;
+    int t = (len + kStep - 1) / kStep;
+    for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o);
+    total += t;
+  }
+  total = __builtin_amdgcn_readfirstlane((int)min(total, 0x7fffffffL));
+  out.steps = max(least, (int)((total + target - 1) / target));
+  int before = 0;
+  for (int base = 0; base < c.batch; base += 64) {
+    if (c.batch > 64) len = base + lane < c.batch ? c.len(base + lane) : 0;
+    const int t = (len + kStep - 1) / kStep;
+    const int n = base + lane < c.batch
+                      ? max(1, (t + out.steps - 1) / out.steps)
+                      : 0;
+    int upto = n;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o);
+      if (lane >= o) upto += x;
     }
-    float top = wave_max(s);
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float mn = fmaxf(m, top);
-    const float safe = mn == -INFINITY ? 0.f : mn;
-    const float r = expf(m - safe);
-    p[tid] = expf(s - safe);
-    m = mn;
-    acc *= r;
-    l *= r;
-    __syncthreads();
-    for (int i = 0; i < 256; ++i) l += p[i];
-    const int top_i = min(256, len - base);
-    for (int i = lane; i < top_i; i += lanes) {
-      if (p[i] == 0.f) continue;  // also a slot whose page is missing
-      const long page = a.c.page(b, base + i);
-      acc += p[i] * (float)((const T *)a.c.v)[page * a.c.v_page +
-                                              ((base + i) % a.c.block) *
-                                                  a.c.v_row +
-                                              kh * a.c.v_head + col];
+    const bool here = id >= 0 ? before + upto > id : base + lane == seq;
+    const unsigned long long found = __ballot(here);
+    if (found) {
+      const int f = __builtin_ctzll(found);
+      out.b = base + f;
+      out.len = __builtin_amdgcn_readlane(len, f);
+      out.count = __builtin_amdgcn_readlane(n, f);
+      const int start = before + __builtin_amdgcn_readlane(upto, f) -
+                        out.count;
+      out.first = id >= 0 ? id - start : 0;
+      out.id = start + out.first;
+      return true;
     }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// Where a call keeps what its kernels hand on.
+struct DecodeWork {
+  float *part;    // [chunks, qh, d]: a chunk's outputs
+  float *sum;     // [chunks, qh]: log2 of a chunk's sum
+  float *logits;  // [batch, qh, room], in units of log2, where weights are
+  int target, least, groups;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 3) void k_paged_decode(PagedDecodeArgs a,
+                                                         DecodeWork w) {
+  constexpr int kC = D / 32, kT = D / 16;  // pieces of a row, tiles of it
+  constexpr int kRow = D + 16;   // of V in LDS: 8 rows take all 64 banks
+  constexpr int kORow = D + 4;   // of the outputs there, floats
+  constexpr int kBytes = kTile * kRow * 2;
+  static_assert(16 * kORow * 4 <= kBytes, "outputs fit where V was");
+  __shared__ __attribute__((aligned(16))) char lds[4][kBytes];
+  __shared__ float lds_m[4][16], lds_l[4][16];
+
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int n = lane & 15, qd = lane >> 4;
+  const int per = a.c.kvh * w.groups;
+  Chunk ch;
+  if (!find_chunk(a.c, w.target, w.least, blockIdx.x / per, 0, ch)) return;
+  const int kh = blockIdx.x % per / w.groups;
+  const int group = blockIdx.x % per % w.groups;
+  const int g = a.qh / a.c.kvh;
+  const int h0 = kh * g + group * 16;       // first query head here
+  const int heads = min(16, g - group * 16);
+  const int b = ch.b;
+  const long cut = (long)ch.steps * kStep;
+  const int k0 = (int)(ch.first * cut);
+  const int k1 = (int)min((long)ch.len, k0 + cut);
+
+  vec8<T> qf[kC] = {};
+  if (n < heads) {
+    const T *q = (const T *)a.q + b * a.q_tok + (h0 + n) * a.q_head + qd * 8;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) qf[c] = *(const vec8<T> *)(q + c * 32);
+  }
+  const float scale = a.s.scale * kLog2e;
+  const float cap = a.s.softcap * kLog2e;
+  const float in_cap = a.s.softcap > 0.f ? 2.f * kLog2e * a.s.scale /
+                                               a.s.softcap : 0.f;
+  const float slope = a.s.slopes && n < heads ? a.s.slopes[h0 + n] * kLog2e
+                                              : 0.f;
+  const int *key_pos = a.key_pos ? a.key_pos + ((long)b * a.c.kvh + kh) *
+                                                   a.c.room()
+                                 : nullptr;
+  const long q_at = key_pos ? a.q_pos[b] : (long)ch.len - 1;
+
+  const T *kbase = (const T *)a.c.k + kh * a.c.k_head + qd * 8;
+  const T *vbase = (const T *)a.c.v + kh * a.c.v_head + qd * 8;
+  vec8<T> kf[2][kC], vf[2][kC];
+  int page[2];     // of the tile to load next
+  bool ok[2];      // this lane's rows of the loaded tile are there
+  auto look_up = [&](int base) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int slot = base + 16 * t + n;
+      page[t] = slot < k1 ? (int)a.c.page(b, slot) : -1;
+    }
+  };
+  // Rows that are not there are read from the pool's first page instead,
+  // masked as keys and cleared as values before they are used.
+  auto load_k = [&](int base) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const long p = max(page[t], 0);
+      const unsigned r = (unsigned)(base + 16 * t + n) % (unsigned)a.c.block;
+      const T *row = kbase + p * a.c.k_page + r * a.c.k_row;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        kf[t][c] = *(const vec8<T> *)(row + c * 32);
+    }
+  };
+  auto load_v = [&](int base) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      ok[t] = page[t] >= 0;
+      const long p = max(page[t], 0);
+      const unsigned r = (unsigned)(base + 16 * t + n) % (unsigned)a.c.block;
+      const T *row = vbase + p * a.c.v_page + r * a.c.v_row;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        vf[t][c] = *(const vec8<T> *)(row + c * 32);
+    }
+  };
+
+  float m = -INFINITY, l = 0.f;  // m of all quads alike, l of this lane
+  f32x4 acc[kT] = {};
+  T *vl = (T *)lds[wave];
+  int base = k0 + wave * kTile;
+  if (base < k1) {
+    look_up(base);
+    load_k(base);
+    load_v(base);
+    look_up(base + kStep);
+  }
+  for (; base < k1; base += kStep) {
+    const bool more = base + kStep < k1;
+    f32x4 s[2] = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < kC; ++c) s[t] = mfma16(kf[t][c], qf[c], s[t]);
+    // which of the tile's 32 rows are there, seen by every lane
+    const unsigned here = (unsigned)(__ballot(ok[0]) & 0xffff) |
+                          (unsigned)(__ballot(ok[1]) & 0xffff) << 16;
+    if (here != 0xffffffffu) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (!ok[t])
+#pragma unroll
+          for (int c = 0; c < kC; ++c) vf[t][c] = vec8<T>{};
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        *(vec8<T> *)(vl + (16 * t + n) * kRow + c * 32 + qd * 8) = vf[t][c];
+    wave_fence();
+    if (more) {
+      load_k(base + kStep);
+      load_v(base + kStep);
+      look_up(base + 2 * kStep);
+    }
+    // scores, in units of log2
+    if (a.s.softcap > 0.f) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[t][i] = cap - 2.f * cap *
+                              __builtin_amdgcn_rcpf(
+                                  1.f + __builtin_amdgcn_exp2f(s[t][i] *
+                                                               in_cap));
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[t] *= scale;
+    }
+    if (a.s.slopes) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int slot = base + 16 * t + 4 * qd + i;
+          long far = slot;
+          if (key_pos) far = key_pos[min(slot, k1 - 1)];
+          far = q_at - far;
+          s[t][i] -= slope * (float)(far < 0 ? -far : far);
+        }
+    }
+    if (here != 0xffffffffu) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(here >> (16 * t + 4 * qd + i) & 1)) s[t][i] = -INFINITY;
+    }
+    if (w.logits && n < heads) {
+      float *to = w.logits + ((long)b * a.qh + h0 + n) * a.c.room() + base;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (base + 16 * t + 4 * qd + i < k1) to[16 * t + 4 * qd + i] =
+              s[t][i];
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]),
+                            fmaxf(s[0][2], s[0][3])),
+                      fmaxf(fmaxf(s[1][0], s[1][1]),
+                            fmaxf(s[1][2], s[1][3])));
+    if (__any(top > m)) {  // seldom after the first tiles
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float to = fmaxf(m, top);
+      const float r = __builtin_amdgcn_exp2f(
+          m - (to == -INFINITY ? 0.f : to));
+      m = to;
+      l *= r;
+#pragma unroll
+      for (int t = 0; t < kT; ++t) acc[t] *= r;
+    }
+    const float safe = m == -INFINITY ? 0.f : m;
+    vec8<T> hi, lo;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(s[t][i] - safe);
+        l += p;
+        hi[4 * t + i] = (T)p;
+        lo[4 * t + i] = (T)(p - (float)hi[4 * t + i]);
+      }
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const T *at = vl + (4 * qd + (n >> 2)) * kRow + t * 16 + 4 * (n & 3);
+      union { s16x4 half[2]; vec8<T> all; } v;
+      v.half[0] = read_transposed(at);
+      v.half[1] = read_transposed(at + 16 * kRow);
+      acc[t] = mfma16(v.all, hi, acc[t]);
+      acc[t] = mfma16(v.all, lo, acc[t]);
+    }
+    wave_fence();  // the next tile's values go where these were
+  }
+
+  // join the four waves
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  float *ol = (float *)lds[wave];
+#pragma unroll
+  for (int t = 0; t < kT; ++t)
+    *(f32x4 *)(ol + n * kORow + t * 16 + qd * 4) = acc[t];
+  if (qd == 0) {
+    lds_m[wave][n] = m;
+    lds_l[wave][n] = l;
   }
   __syncthreads();
-  part[tid] = acc;
-  __syncthreads();
-  if (tid < d) {
-    for (int i = 1; i < lanes; ++i) acc += part[i * d + tid];
-    ((T *)a.out)[((long)b * a.qh + h) * d + tid] =
-        (T)(l > 0.f ? acc / l : 0.f);
-    if (tid == 0)
-      a.lse[(long)b * a.qh + h] = l > 0.f ? m + logf(l) : -INFINITY;
+  for (int i = tid; i < heads * (D / 4); i += 256) {
+    const int h = i / (D / 4), c = i % (D / 4) * 4;
+    const float top = fmaxf(fmaxf(lds_m[0][h], lds_m[1][h]),
+                            fmaxf(lds_m[2][h], lds_m[3][h]));
+    const float safe = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    f32x4 o = {};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float r = __builtin_amdgcn_exp2f(lds_m[x][h] - safe);
+      sum += r * lds_l[x][h];
+      o += r * *(const f32x4 *)((const float *)lds[x] + h * kORow + c);
+    }
+    o *= sum == 0.f ? 0.f : 1.f / sum;
+    const float lse = sum == 0.f ? -INFINITY
+                                 : top + __builtin_amdgcn_logf(sum);
+    if (ch.count == 1) {
+      T *to = (T *)a.out + ((long)b * a.qh + h0 + h) * D + c;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) to[x] = (T)o[x];
+      if (c == 0) a.lse[(long)b * a.qh + h0 + h] = lse * kLn2;
+    } else {
+      const long at = (long)ch.id * a.qh + h0 + h;
+      *(f32x4 *)(w.part + at * D + c) = o;
+      if (c == 0) w.sum[at] = lse;
+    }
   }
 }
 
-// The weights that the query heads of a key head gave each slot.
-template <typename T>
-__global__ __launch_bounds__(256) void k_paged_mass(PagedDecodeArgs a) {
-  extern __shared__ float qs[];
+// Joins the chunks of a sequence's query head: a wave each.
+template <typename T, int D>
+__global__ __launch_bounds__(64) void k_decode_join(PagedDecodeArgs a,
+                                                    DecodeWork w) {
+  Chunk ch;
+  const int h = blockIdx.y, lane = threadIdx.x;
+  find_chunk(a.c, w.target, w.least, -1, blockIdx.x, ch);
+  if (ch.count == 1) return;
+  const float *sum = w.sum + (long)ch.id * a.qh + h;
+  const float *part = w.part + ((long)ch.id * a.qh + h) * D + lane * (D / 64);
+  float top = -INFINITY;
+  for (int i = lane; i < ch.count; i += 64)
+    top = fmaxf(top, sum[(long)i * a.qh]);
+  top = wave_max(top);
+  const float safe = top == -INFINITY ? 0.f : top;
+  float total = 0.f, o[D / 64] = {};
+  for (int i = 0; i < ch.count; ++i) {
+    const float r = __builtin_amdgcn_exp2f(sum[(long)i * a.qh] - safe);
+    total += r;
+#pragma unroll
+    for (int x = 0; x < D / 64; ++x)
+      o[x] += r * part[(long)i * a.qh * D + x];
+  }
+  const float f = total == 0.f ? 0.f : 1.f / total;
+  T *out = (T *)a.out + ((long)ch.b * a.qh + h) * D + lane * (D / 64);
+#pragma unroll
+  for (int x = 0; x < D / 64; ++x) out[x] = (T)(o[x] * f);
+  if (lane == 0)
+    a.lse[(long)ch.b * a.qh + h] =
+        total == 0.f ? -INFINITY
+                     : (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+// The weights that the query heads of a key head gave each slot, from the
+// logits that the first kernel kept.
+__global__ __launch_bounds__(256) void k_decode_mass(PagedDecodeArgs a,
+                                                     DecodeWork w) {
   const int b = blockIdx.y, kh = blockIdx.z, g = a.qh / a.c.kvh;
-  const int d = a.c.d, slot = blockIdx.x * 256 + threadIdx.x;
-  for (int i = threadIdx.x; i < g * d; i += 256)
-    qs[i] = (float)((const T *)a.q)[b * a.q_tok + (kh * g + i / d) *
-                                                      a.q_head + i % d];
-  __syncthreads();
-  const int len = a.c.len(b);
-  if (slot >= a.c.room()) return;
-  const long at = ((long)b * a.c.kvh + kh) * a.c.room() + slot;
-  if (slot >= len) {
-    a.mass_out[at] = 0.f;
-    return;
-  }
-  float w = 0.f;
-  const long page = a.c.page(b, slot);
-  if (page >= 0)
+  const int slot = blockIdx.x * 256 + threadIdx.x, room = a.c.room();
+  if (slot >= room) return;
+  const long at = ((long)b * a.c.kvh + kh) * room + slot;
+  float m = 0.f;
+  if (slot < a.c.len(b)) {
+    m = a.mass[at];
+    const float *s = w.logits + ((long)b * a.qh + kh * g) * room + slot;
+    const float *lse = a.lse + (long)b * a.qh + kh * g;
+    float sum = 0.f;
     for (int i = 0; i < g; ++i) {
-      const float lse = a.lse[(long)b * a.qh + kh * g + i];
-      if (lse == -INFINITY) continue;
-      w += expf(score<T>(a, qs + i * d, b, kh * g + i, slot, len, page) -
-                lse);
+      const float x = lse[i];
+      if (x != -INFINITY)
+        sum += __builtin_amdgcn_exp2f(s[(long)i * room] - x * kLog2e);
     }
-  a.mass_out[at] = a.mass[at] + w;
+    m += sum;
+  }
+  a.mass_out[at] = m;
 }
 
 // ---------------------------------------------------------------------------
@@ -315,19 +617,57 @@ void launch_paged_append(const PagedArgs &a, const void *k, long k_tok,
   launched("paged_append");
 }
 
-size_t paged_decode_workspace(int, int, int, int, long, bool) { return 0; }
+// Chunks are made so that the card is full: kSlots workgroups, of which
+// each sequence may add one that is not.
+static DecodeWork decode_work(int batch, int qh, int kvh) {
+  DecodeWork w{};
+  w.groups = (qh / kvh + 15) / 16;
+  const int per = kvh * w.groups;
+  w.target = (kSlots + per - 1) / per;
+  w.least = 2;
+  return w;
+}
+
+size_t paged_decode_workspace(int batch, int qh, int kvh, int d, long room,
+                              bool mass) {
+  const DecodeWork w = decode_work(batch, qh, kvh);
+  const size_t chunks = (size_t)w.target + batch;
+  return (chunks * qh * (d + 1) + (mass ? (size_t)batch * qh * room : 0)) *
+         sizeof(float);
+}
+
+template <typename T, int D>
+static void decode(const PagedDecodeArgs &a, const DecodeWork &w,
+                   hipStream_t stream) {
+  const long blocks = ((long)w.target + a.c.batch) * a.c.kvh * w.groups;
+  if (blocks > 0x7fffffffL)
+    throw std::runtime_error("paged_decode: too many sequences and heads");
+  k_paged_decode<T, D><<<dim3((unsigned)blocks), 256, 0, stream>>>(a, w);
+  launched("paged_decode");
+  if (a.c.room() > w.least * kStep) {  // else no sequence has two chunks
+    k_decode_join<T, D><<<dim3(a.c.batch, a.qh), 64, 0, stream>>>(a, w);
+    launched("paged_decode");
+  }
+}
 
 void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
   if (!a.c.batch) return;
-  const dim3 grid(a.c.batch, a.qh);
-  if (a.c.is_fp16) k_paged_decode<_Float16><<<grid, 256, 0, stream>>>(a);
-  else k_paged_decode<bf16><<<grid, 256, 0, stream>>>(a);
-  launched("paged_decode");
+  if (a.c.batch > 65535 || a.c.kvh > 65535)
+    throw std::runtime_error("paged_decode: 65535 sequences and heads at most");
+  DecodeWork w = decode_work(a.c.batch, a.qh, a.c.kvh);
+  w.part = (float *)a.ws;
+  w.sum = w.part + ((size_t)w.target + a.c.batch) * a.qh * a.c.d;
+  w.logits = a.mass ? w.sum + ((size_t)w.target + a.c.batch) * a.qh
+                    : nullptr;
+  if (a.c.is_fp16)
+    a.c.d == 64 ? decode<_Float16, 64>(a, w, stream)
+                : decode<_Float16, 128>(a, w, stream);
+  else
+    a.c.d == 64 ? decode<bf16, 64>(a, w, stream)
+                : decode<bf16, 128>(a, w, stream);
   if (a.mass && a.c.room()) {
-    const dim3 mg((a.c.room() + 255) / 256, a.c.batch, a.c.kvh);
-    const size_t lds = (size_t)(a.qh / a.c.kvh) * a.c.d * 4;
-    if (a.c.is_fp16) k_paged_mass<_Float16><<<mg, 256, lds, stream>>>(a);
-    else k_paged_mass<bf16><<<mg, 256, lds, stream>>>(a);
+    const dim3 grid((a.c.room() + 255) / 256, a.c.batch, a.c.kvh);
+    k_decode_mass<<<grid, 256, 0, stream>>>(a, w);
     launched("paged_decode");
   }
 }

@@ -94,6 +94,7 @@ def _cache(k_pool, v_pool, block_table, seq_lens):
           "v_pool: of k_pool's type, shape and device")
     n, block, kvh, d = k_pool.shape
     _need(block >= 1 and kvh >= 1, "k_pool: empty blocks")
+    _need(1 <= n < 1 << 31, f"k_pool: from 1 to 2^31 - 1 pages, got {n}")
     _need(d % 8 == 0 and d >= 8, f"k_pool: d a multiple of 8, got {d}")
     _rows16("k_pool", k_pool)
     _rows16("v_pool", v_pool)
@@ -198,7 +199,7 @@ def paged_append_op(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
     if key_pos is not None:
         _plane("key_pos", key_pos, torch.int32, (b, kvh, room), dev)
         _index("pos", pos, (tokens,), dev)
-    if not tokens or not b or not n:
+    if not tokens or not b:
         return
     if k_pool.is_cuda:
         with torch.cuda.device(dev):
