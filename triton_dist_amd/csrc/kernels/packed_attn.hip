@@ -55,13 +55,6 @@ TD_DEV s16x4 read_transposed(const void *lds) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
       (__attribute__((address_space(3))) s16x4 *)(unsigned)(uintptr_t)lds);
 }
-// 16 bytes from `from` to this lane's place behind the wave's `to`.
-TD_DEV void load_to_lds(const void *from, void *to) {
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) unsigned *)from,
-      (__attribute__((address_space(3))) unsigned *)to, 16, 0, 0);
-}
-
 // Where a row's 16-byte pieces lie in LDS. K: eight rows' pieces of one
 // column take all banks. V: the 64 bytes of four rows that 32 lanes read
 // transposed do.
@@ -205,27 +198,39 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   const T *kbase = (const T *)a.k + doc.k0 * a.k_tok + kh * a.k_head;
   const T *vbase = (const T *)a.v + doc.k0 * a.v_tok + kh * a.v_head;
   // Keys past the document repeat its last one: their weights are zero.
-  auto stage = [&](int step, int buf) {
+  vec8<T> nk[kLoads], nv[kLoads];
+  auto fetch = [&](int step) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int at16 = (i * kWaves + wave) * 64;
-      const int r = (at16 + lane) / kP, p = (at16 + lane) % kP;
+      const int r = (i * 64 * kWaves + tid) / kP, p = tid % kP;
       const long key = min(step * kKeys + r, doc.n - 1);
-      load_to_lds(kbase + key * a.k_tok + k_piece<D>(r, p) * 8,
-                  &lds_k[buf][at16 * 8]);
-      load_to_lds(vbase + key * a.v_tok + v_piece<D>(r, p) * 8,
-                  &lds_v[buf][at16 * 8]);
+      nk[i] = *(const vec8<T> *)(kbase + key * a.k_tok + p * 8);
+      nv[i] = *(const vec8<T> *)(vbase + key * a.v_tok + p * 8);
+    }
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (i * 64 * kWaves + tid) / kP, p = tid % kP;
+      *(vec8<T> *)&lds_k[buf][r * D + k_piece<D>(r, p) * 8] = nk[i];
+      *(vec8<T> *)&lds_v[buf][r * D + v_piece<D>(r, p) * 8] = nv[i];
     }
   };
 
   float m = -INFINITY, l = 0.f;
   f32x16 acc[D / 32] = {};
-  if (steps) stage(0, 0);
+  if (steps) {
+    fetch(0);
+    stage(0);
+    if (steps > 1) fetch(1);
+  }
   for (int step = 0; step < steps; ++step) {
     const int buf = step & 1, base = step * kKeys;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // this step is there, the other buffer is free
-    if (step + 1 < steps) stage(step + 1, buf ^ 1);
+    if (step + 1 < steps) {
+      stage(buf ^ 1);
+      if (step + 2 < steps) fetch(step + 2);
+    }
     if (base >= most) continue;
     f32x16 s[2] = {};
 #pragma unroll
