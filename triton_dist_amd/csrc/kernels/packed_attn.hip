@@ -55,15 +55,12 @@ TD_DEV s16x4 read_transposed(const void *lds) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
       (__attribute__((address_space(3))) s16x4 *)(unsigned)(uintptr_t)lds);
 }
-// Where a row's 16-byte pieces lie in LDS. K: eight rows' pieces of one
-// column take all banks. V: the 64 bytes of four rows that 32 lanes read
-// transposed do.
-template <int D> TD_DEV int k_piece(int row, int piece) {
-  return piece ^ (row & (D / 8 - 1));
-}
-template <int D> TD_DEV int v_piece(int row, int piece) {
-  return D == 128 ? piece ^ (row & 3) << 2 : piece ^ (row >> 1 & 1) << 2;
-}
+// Elements from row to row in LDS. K: 16 bytes more than a row, so that the
+// same piece of eight rows takes different banks. V: 64 bytes more, so that
+// the 64 bytes of four rows that 32 lanes read transposed do. With fixed
+// steps every read of a step is one address and an offset.
+template <int D> constexpr int kRowK = D + 8;
+template <int D> constexpr int kRowV = D + 32;
 
 struct Doc {
   long q0, k0;
@@ -131,10 +128,9 @@ template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
     PackedArgs a, int tiles) {
   constexpr int kP = D / 8;          // 16-byte pieces of a row
-  constexpr int kStage = kKeys * D;  // elements of a staged K or V
   constexpr int kLoads = kKeys * kP / (64 * kWaves);
-  __shared__ __attribute__((aligned(16))) T lds_k[2][kStage];
-  __shared__ __attribute__((aligned(16))) T lds_v[2][kStage];
+  __shared__ __attribute__((aligned(16))) T lds_k[2][kKeys * kRowK<D>];
+  __shared__ __attribute__((aligned(16))) T lds_v[2][kKeys * kRowV<D>];
   __shared__ int lds_see[kWaves];
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -162,6 +158,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
       lim = max(lim, (int)min(a.prefix[doc.index], (long)doc.n));
   }
   if (!live) lim = 0;
+  const bool only_back = a.causal && !a.prefix.p;
+  const int first_pos = row0 + doc.n - doc.m;
   int most = lim, least = lim;
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -186,101 +184,113 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
       if (a.s.scale == 0.f) qf[s] = vec8<T>{};
     }
   }
-  const float cap = a.s.softcap * kLog2e;
+  // A logit in units of log2 is cf x + c0, less slope times the distance:
+  // x is the score itself, or with a cap 1 / (1 + e^(2 s / cap)), of which
+  // cap tanh is cap - 2 cap x.
+  const float cf = CAP ? -2.f * kLog2e * a.s.softcap : c1;
+  const float c0 = CAP ? kLog2e * a.s.softcap : 0.f;
   const float in_cap = CAP ? 2.f * c1 / a.s.softcap : 0.f;
+  // The distance to key 4 h + 8 (r / 4) + r % 4 of 32 is gap less that, so
+  // what a lane's 16 keys differ by is the same for the whole wave.
   const float slope = BIAS ? a.s.slopes[head] * kLog2e : 0.f;
+  float step_up[BIAS ? 16 : 1];
+  if (BIAS)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      step_up[r] = __uint_as_float(__builtin_amdgcn_readfirstlane(
+          __float_as_uint(slope * (float)(8 * (r / 4) + r % 4))));
   __syncthreads();
   int see = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) see = max(see, lds_see[w]);
   const int steps = (see + kKeys - 1) / kKeys;
 
-  const T *kbase = (const T *)a.k + doc.k0 * a.k_tok + kh * a.k_head;
-  const T *vbase = (const T *)a.v + doc.k0 * a.v_tok + kh * a.v_head;
   // Keys past the document repeat its last one: their weights are zero.
+  constexpr int kPer = 64 * kWaves / kP;  // rows that the workgroup moves
+  const int srow = tid / kP, piece = tid % kP;
+  const T *kfrom = (const T *)a.k + doc.k0 * a.k_tok + kh * a.k_head +
+                   piece * 8;
+  const T *vfrom = (const T *)a.v + doc.k0 * a.v_tok + kh * a.v_head +
+                   piece * 8;
   vec8<T> nk[kLoads], nv[kLoads];
-  auto fetch = [&](int step) {
+  auto fetch = [&](vec8<T> *to, const T *from, long tok, int first) {
+    if (first >= see) return;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = (i * 64 * kWaves + tid) / kP, p = tid % kP;
-      const long key = min(step * kKeys + r, doc.n - 1);
-      nk[i] = *(const vec8<T> *)(kbase + key * a.k_tok + p * 8);
-      nv[i] = *(const vec8<T> *)(vbase + key * a.v_tok + p * 8);
+      const int key = max(0, min(first + i * kPer + srow, doc.n - 1));
+      to[i] = *(const vec8<T> *)(from + key * tok);
     }
   };
-  auto stage = [&](int buf) {
+  auto stage_k = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = (i * 64 * kWaves + tid) / kP, p = tid % kP;
-      *(vec8<T> *)&lds_k[buf][r * D + k_piece<D>(r, p) * 8] = nk[i];
-      *(vec8<T> *)&lds_v[buf][r * D + v_piece<D>(r, p) * 8] = nv[i];
+      const int r = i * kPer + srow;
+      *(vec8<T> *)&lds_k[buf][r * kRowK<D> + piece * 8] = nk[i];
+    }
+  };
+  auto stage_v = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * kPer + srow;
+      *(vec8<T> *)&lds_v[buf][r * kRowV<D> + piece * 8] = nv[i];
     }
   };
 
   float m = -INFINITY, l = 0.f;
   f32x16 acc[D / 32] = {};
-  if (steps) {
-    fetch(0);
-    stage(0);
-    if (steps > 1) fetch(1);
-  }
-  for (int step = 0; step < steps; ++step) {
-    const int buf = step & 1, base = step * kKeys;
-    __syncthreads();  // this step is there, the other buffer is free
-    if (step + 1 < steps) {
-      stage(buf ^ 1);
-      if (step + 2 < steps) fetch(step + 2);
+  const int kread = c * kRowK<D> + h * 8;
+  const int vread = (4 * h + ((lane & 15) >> 2)) * kRowV<D> + (lane & 16) +
+                    4 * (lane & 3);
+  auto k_frag = [&](int buf, int sub, int x) {
+    return *(const vec8<T> *)(&lds_k[0][buf * kKeys * kRowK<D> + kread +
+                                        32 * sub * kRowK<D> + 16 * x]);
+  };
+  auto v_frag = [&](int buf, int sub, int j) {
+    constexpr int n = D / 32;
+    union { s16x4 half[2]; vec8<T> all; } v;
+    const T *at = &lds_v[0][buf * kKeys * kRowV<D> + vread +
+                            (32 * sub + 16 * (j / n)) * kRowV<D> +
+                            32 * (j % n)];
+    v.half[0] = read_transposed(at);
+    v.half[1] = read_transposed(at + 8 * kRowV<D>);
+    return v.all;
+  };
+  // What is kept of a score until it is weighed: x, or with a bias the logit
+  // but for c0 and slope times gap.
+  auto keep = [&](float x, int r) {
+    if (CAP)
+      x = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * in_cap));
+    return BIAS ? x * cf + step_up[r] : x;
+  };
+  constexpr bool kLow = CAP && !BIAS;  // a small x is a large logit
+  constexpr float kHidden = kLow ? INFINITY : -INFINITY;
+  auto larger = [](float x, float y) {
+    return kLow ? fminf(x, y) : fmaxf(x, y);
+  };
+  // Slope times gap, for the 32 keys from `base` on.
+  auto lean = [&](int base) {
+    return BIAS ? slope * (float)(pos - base - 4 * h) : 0.f;
+  };
+  // Where not all of the wave's rows see the 32 keys from `base` on, hides
+  // what they do not see; where keys behind a row are seen, turns their
+  // distance's sign. Then finds the largest again.
+  auto mend = [&](f32x16 &s, int base, float &top) {
+    const bool turn = BIAS && !only_back && base + 32 > first_pos;
+    if (base + 32 <= least && !turn) return;
+    const int left = lim - base - 4 * h, gap = pos - base - 4 * h;
+    top = kHidden;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = 8 * (r / 4) + r % 4;
+      if (BIAS && j > gap) s[r] -= 2.f * slope * (float)(j - gap);
+      if (j >= left) s[r] = kHidden;
+      top = larger(top, s[r]);
     }
-    if (base >= most) continue;
-    f32x16 s[2] = {};
-#pragma unroll
-    for (int x = 0; x < D / 16; ++x)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int r = 32 * t + c;
-        const vec8<T> kf = *(const vec8<T> *)(
-            &lds_k[buf][r * D + k_piece<D>(r, 2 * x + h) * 8]);
-        s[t] = mfma32(kf, qf[x], s[t]);
-      }
-    if (CAP) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[t][r] = cap - 2.f * cap *
-                              __builtin_amdgcn_rcpf(
-                                  1.f + __builtin_amdgcn_exp2f(s[t][r] *
-                                                               in_cap));
-    }
-    if (BIAS) {
-      const float gap = (float)(pos - base - 4 * h);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float z = CAP ? s[t][r] : s[t][r] * c1;
-          const float far = gap - (float)(32 * t + 8 * (r / 4) + r % 4);
-          s[t][r] = z - slope * fabsf(far);
-        }
-    }
-    if (base + kKeys > least) {  // not all of the wave's rows see all keys
-      const int left = lim - base - 4 * h;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * t + 8 * (r / 4) + r % 4 >= left) s[t][r] = -INFINITY;
-    }
-    // plain scores are scaled in the exponent's multiply-add
-    const float f = CAP || BIAS ? 1.f : c1;
-    float top = s[0][0];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-    top = fmaxf(top, __shfl_xor(top, 32)) * f;
+  };
+  auto raise = [&](float top, int base) {
+    top = BIAS ? top + (c0 - lean(base)) : top * cf + c0;
     if (__any(top > m + kSlack)) {
-      const float to = fmaxf(m, top);
+      const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
       const float x = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f
                                                                   : to));
       m = to;
@@ -288,30 +298,96 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
 #pragma unroll
       for (int t = 0; t < D / 32; ++t) acc[t] *= x;
     }
-    const float safe = m == -INFINITY ? 0.f : m;
-    vec8<T> p[4];
+  };
+  // 32 keys' scores in `s` are weighed and their values collected while the
+  // next 32 keys' scores are made in `next`, `base` on. The order is written
+  // out, so that reads run two or three products ahead and each product of
+  // 32 cycles has about as much vector work beside it: the weights beside
+  // the scores' products, the next logits beside the values'.
+  auto work = [&](f32x16 &s, f32x16 &next, int step, int sub) {
+    constexpr int nx = D / 16, nj = D / 16;
+    const int buf = step & 1, base = step * kKeys + 32 * (sub + 1);
+    const float from = c0 - lean(base - 32) - (m == -INFINITY ? 0.f : m);
+    vec8<T> kq[3], vq[3], p[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int x = 0; x < 3; ++x) kq[x] = k_frag(buf, sub, x);
+    // behind the last keys the products are of no use and no harm
+#pragma unroll
+    for (int x = 0; x < nx; ++x) {
+      __builtin_amdgcn_sched_barrier(0);
+      next = mfma32(kq[x % 3], qf[x], x ? next : f32x16{});
+      if (x + 3 < nx) kq[x % 3] = k_frag(buf, sub, x + 3);
+      else vq[x + 3 - nx] = v_frag(buf, sub, x + 3 - nx);
+#pragma unroll
+      for (int r = 16 / nx * x; r < 16 / nx * (x + 1); ++r) {
+        const float e =
+            __builtin_amdgcn_exp2f(BIAS ? s[r] + from : s[r] * cf + from);
+        l += e;
+        p[r / 8][r % 8] = (T)e;
+      }
+    }
+    float top = kHidden;
+#pragma unroll
+    for (int j = 0; j < nj; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      acc[j % (D / 32)] = mfma32(vq[j % 3], p[j / (D / 32)],
+                                 acc[j % (D / 32)]);
+      if (j + 3 < nj) vq[j % 3] = v_frag(buf, sub, j + 3);
+      if (j < 2) continue;  // the scores are still on their way
+#pragma unroll
+      for (int r = 16 * (j - 2) / (nj - 2); r < 16 * (j - 1) / (nj - 2);
+           ++r) {
+        next[r] = keep(next[r], r);
+        top = larger(top, next[r]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (base < most) {
+      mend(next, base, top);
+      raise(top, base);
+    }
+  };
+
+  // A step's V are the keys from 64 step on; its K are those of the
+  // products made in it, 32 keys further.
+  f32x16 sa, sb;
+  if (steps) {
+    fetch(nk, kfrom, a.k_tok, -32);
+    fetch(nv, vfrom, a.v_tok, 0);
+    stage_k(1);
+    stage_v(0);
+    fetch(nk, kfrom, a.k_tok, 32);
+    stage_k(0);
+    fetch(nk, kfrom, a.k_tok, kKeys + 32);
+    fetch(nv, vfrom, a.v_tok, kKeys);
+    __syncthreads();
+    if (most > 0) {
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x)
+        sa = mfma32(k_frag(1, 1, x), qf[x], x ? sa : f32x16{});
+      float top = kHidden;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float e = __builtin_amdgcn_exp2f(s[t][r] * f - safe);
-        l += e;
-        p[2 * t + r / 8][r % 8] = (T)e;
+        sa[r] = keep(sa[r], r);
+        top = larger(top, sa[r]);
       }
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t) {
-        const int r = 16 * x + 4 * h + ((lane & 15) >> 2);
-        const int col = 32 * t + (lane & 16) + 4 * (lane & 3);
-        union { s16x4 half[2]; vec8<T> all; } v;
-        v.half[0] = read_transposed(
-            &lds_v[buf][r * D + v_piece<D>(r, col / 8) * 8 + col % 8]);
-        v.half[1] = read_transposed(
-            &lds_v[buf][(r + 8) * D + v_piece<D>(r + 8, col / 8) * 8 +
-                        col % 8]);
-        acc[t] = mfma32(v.all, p[x], acc[t]);
-      }
+      mend(sa, 0, top);
+      raise(top, 0);
+    }
+  }
+  for (int step = 0; step < steps; ++step) {
+    const int base = step * kKeys;
+    __syncthreads();  // this step is there, the other buffers are free
+    if (step + 1 < steps) {
+      stage_k((step & 1) ^ 1);
+      stage_v((step & 1) ^ 1);
+      fetch(nk, kfrom, a.k_tok, base + 2 * kKeys + 32);
+      fetch(nv, vfrom, a.v_tok, base + 2 * kKeys);
+    }
+    if (base < most) {
+      work(sa, sb, step, 0);
+      if (base + 32 < most) work(sb, sa, step, 1);
+    }
   }
   if (!live || row0 + c >= doc.m) return;
   l += __shfl_xor(l, 32);
