@@ -187,7 +187,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   // A logit in units of log2 is cf x + c0, less slope times the distance:
   // x is the score itself, or with a cap 1 / (1 + e^(2 s / cap)), of which
   // cap tanh is cap - 2 cap x.
-  const float cf = CAP ? -2.f * kLog2e * a.s.softcap : c1;
+  float cf = CAP ? -2.f * kLog2e * a.s.softcap : c1;
   const float c0 = CAP ? kLog2e * a.s.softcap : 0.f;
   const float in_cap = CAP ? 2.f * c1 / a.s.softcap : 0.f;
   // The distance to key 4 h + 8 (r / 4) + r % 4 of 32 is gap less that, so
@@ -199,6 +199,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
     for (int r = 0; r < 16; ++r)
       step_up[r] = __uint_as_float(__builtin_amdgcn_readfirstlane(
           __float_as_uint(slope * (float)(8 * (r / 4) + r % 4))));
+  // an instruction takes one scalar register: leave it to these
+  asm("" : "+v"(cf));
   __syncthreads();
   int see = 0;
 #pragma unroll
