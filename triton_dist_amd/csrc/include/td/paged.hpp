@@ -70,7 +70,7 @@ struct PagedDecodeArgs {
   const int *key_pos;  // [batch, kvh, room] or null
   IdxPtr q_pos;        // [batch], read where key_pos is
   void *out;           // [batch, qh, d]
-  float *lse;          // [batch, qh]
+  float *lse;          // [batch, qh] or null
   const float *mass;   // [batch, kvh, room] or null
   float *mass_out;     // [batch, kvh, room], may be mass itself
   void *ws;

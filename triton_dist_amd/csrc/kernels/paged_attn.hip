@@ -632,7 +632,8 @@ size_t paged_decode_workspace(int batch, int qh, int kvh, int d, long room,
                               bool mass) {
   const DecodeWork w = decode_work(batch, qh, kvh);
   const size_t chunks = (size_t)w.target + batch;
-  return (chunks * qh * (d + 1) + (mass ? (size_t)batch * qh * room : 0)) *
+  return (chunks * qh * (d + 1) + (size_t)batch * qh +
+          (mass ? (size_t)batch * qh * room : 0)) *
          sizeof(float);
 }
 
@@ -650,15 +651,17 @@ static void decode(const PagedDecodeArgs &a, const DecodeWork &w,
   }
 }
 
-void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
+void launch_paged_decode(const PagedDecodeArgs &args, hipStream_t stream) {
+  PagedDecodeArgs a = args;
   if (!a.c.batch) return;
   if (a.c.batch > 65535 || a.c.kvh > 65535)
     throw std::runtime_error("paged_decode: 65535 sequences and heads at most");
   DecodeWork w = decode_work(a.c.batch, a.qh, a.c.kvh);
   w.part = (float *)a.ws;
   w.sum = w.part + ((size_t)w.target + a.c.batch) * a.qh * a.c.d;
-  w.logits = a.mass ? w.sum + ((size_t)w.target + a.c.batch) * a.qh
-                    : nullptr;
+  float *lse = w.sum + ((size_t)w.target + a.c.batch) * a.qh;
+  if (!a.lse) a.lse = lse;
+  w.logits = a.mass ? lse + (size_t)a.c.batch * a.qh : nullptr;
   if (a.c.is_fp16)
     a.c.d == 64 ? decode<_Float16, 64>(a, w, stream)
                 : decode<_Float16, 128>(a, w, stream);

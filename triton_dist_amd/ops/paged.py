@@ -21,16 +21,14 @@ from typing import Optional, Tuple
 
 import torch
 
-_INDEX = (torch.int32, torch.int64)
-_HALF = (torch.bfloat16, torch.float16)
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_BF16, _FP16 = torch.bfloat16, torch.float16
+# the stream as a number, without a Stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream \
+    if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
-def _need(ok: bool, message: str):
-    if not ok:
-        raise ValueError(message)
-
-
-def _C():
+def _native():
     from .. import _C as mod
 
     if mod is None:
@@ -38,38 +36,61 @@ def _C():
     return mod
 
 
-def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("this operator has no backward: call it under "
-                           "torch.no_grad() or detach its inputs")
+def _call(name: str, dev: torch.device, *args):
+    """The native function on the tensors' device and its current stream."""
+    fn = getattr(_native(), name)
+    if dev.index == torch.cuda.current_device():
+        fn(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            fn(*args, _raw_stream(dev.index))
+
+
+# Every check costs host time that a decode step of a few microseconds
+# waits for, so the common case goes by in one comparison or two and
+# messages are put together when they are needed.
+def _refuse(message: str):
+    raise ValueError(message)
+
+
+def _no_backward():
+    raise RuntimeError("this operator has no backward: call it under "
+                       "torch.no_grad() or detach its inputs")
 
 
 def _rows16(name: str, t: torch.Tensor):
     """The kernels move rows in pieces of 16 bytes."""
     if t.numel() == 0:
         return
-    _need(t.stride(-1) == 1 or t.shape[-1] == 1,
-          f"{name}: the last dimension has to be contiguous")
-    _need(all(st % 8 == 0 for st, n in zip(t.stride()[:-1], t.shape[:-1])
-              if n > 1) and t.data_ptr() % 16 == 0,
-          f"{name}: rows have to start at multiples of 16 bytes")
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        _refuse(f"{name}: the last dimension has to be contiguous")
+    if t.data_ptr() % 16 or any(
+            st % 8 and n > 1 for st, n in zip(t.stride()[:-1], t.shape)):
+        _refuse(f"{name}: rows have to start at multiples of 16 bytes")
 
 
-def _index(name: str, t: torch.Tensor, shape, device):
-    _need(t.dtype in _INDEX, f"{name}: int32 or int64, got {t.dtype}")
-    _need(tuple(t.shape) == tuple(shape),
-          f"{name}: shape {tuple(shape)}, got {tuple(t.shape)}")
-    _need(t.device == device, f"{name}: on {t.device}, not on {device}")
-    _need(t.is_contiguous(), f"{name}: has to be contiguous")
+def _heads(name: str, t: torch.Tensor, dtype, dev):
+    """A tensor [tokens, heads, d] beside others of `dtype` on `dev`."""
+    if t.dtype != dtype:
+        _refuse(f"{name}: {dtype} as the others, got {t.dtype}")
+    if t.device != dev:
+        _refuse(f"{name}: on {t.device}, not on {dev}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s0 | s1) & 7 or t.data_ptr() & 15:
+        _rows16(name, t)
 
 
-def _plane(name: str, t: torch.Tensor, dtype, shape, device):
-    _need(t.dtype == dtype, f"{name}: {dtype}, got {t.dtype}")
-    _need(tuple(t.shape) == tuple(shape),
-          f"{name}: shape {tuple(shape)}, got {tuple(t.shape)}")
-    _need(t.device == device, f"{name}: on {t.device}, not on {device}")
-    _need(t.is_contiguous(), f"{name}: has to be contiguous")
+def _array(name: str, t: torch.Tensor, dtype, shape, dev):
+    """Contiguous, of a type (None: a whole number's) and shape."""
+    if t.dtype != dtype and (dtype is not None or t.dtype != _I32
+                             and t.dtype != _I64):
+        _refuse(f"{name}: {dtype or 'int32 or int64'}, got {t.dtype}")
+    if t.shape != shape:
+        _refuse(f"{name}: shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != dev:
+        _refuse(f"{name}: on {t.device}, not on {dev}")
+    if not t.is_contiguous():
+        _refuse(f"{name}: has to be contiguous")
 
 
 def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
@@ -85,41 +106,43 @@ def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
 
 
 def _cache(k_pool, v_pool, block_table, seq_lens):
-    """Checks a cache's layer; returns (n_blocks, block, kvh, d, B, room)."""
-    _need(k_pool.dim() == 4, "k_pool: [n_blocks, block, kvh, d]")
-    _need(k_pool.dtype in _HALF,
-          f"k_pool: bfloat16 or float16, got {k_pool.dtype}")
-    _need(v_pool.dtype == k_pool.dtype and v_pool.shape == k_pool.shape
-          and v_pool.device == k_pool.device,
-          "v_pool: of k_pool's type, shape and device")
-    n, block, kvh, d = k_pool.shape
-    _need(block >= 1 and kvh >= 1, "k_pool: empty blocks")
-    _need(1 <= n < 1 << 31, f"k_pool: from 1 to 2^31 - 1 pages, got {n}")
-    _need(d % 8 == 0 and d >= 8, f"k_pool: d a multiple of 8, got {d}")
-    _rows16("k_pool", k_pool)
-    _rows16("v_pool", v_pool)
-    _need(block_table.dim() == 2, "block_table: [B, max_blocks]")
-    _need(block_table.dtype in _INDEX,
-          f"block_table: int32 or int64, got {block_table.dtype}")
-    _need(block_table.device == k_pool.device,
-          f"block_table: on {block_table.device}, not on {k_pool.device}")
+    """Checks a cache's layer; returns what the native functions want of it
+    and (block, kvh, d, B, slots of a sequence)."""
+    dtype, dev, shape = k_pool.dtype, k_pool.device, k_pool.shape
+    if len(shape) != 4:
+        _refuse("k_pool: [n_blocks, block, kvh, d]")
+    if dtype != _BF16 and dtype != _FP16:
+        _refuse(f"k_pool: bfloat16 or float16, got {dtype}")
+    if v_pool.dtype != dtype or v_pool.shape != shape or v_pool.device != dev:
+        _refuse("v_pool: of k_pool's type, shape and device")
+    n, block, kvh, d = shape
+    if not (0 < n < 1 << 31 and block > 0 and kvh > 0 and d > 0) or d & 7:
+        _refuse("k_pool: from 1 to 2^31 - 1 pages of at least one slot and "
+                f"head, d a multiple of 8, got {tuple(shape)}")
+    k, v = k_pool.data_ptr(), v_pool.data_ptr()
+    k0, k1, k2, k3 = k_pool.stride()
+    v0, v1, v2, v3 = v_pool.stride()
+    if k3 != 1 or v3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & 7 \
+            or (k | v) & 15:
+        _rows16("k_pool", k_pool)
+        _rows16("v_pool", v_pool)
+    if block_table.dim() != 2:
+        _refuse("block_table: [B, max_blocks]")
+    if block_table.dtype != _I64 and block_table.dtype != _I32:
+        _refuse(f"block_table: int32 or int64, got {block_table.dtype}")
+    if block_table.device != dev:
+        _refuse(f"block_table: on {block_table.device}, not on {dev}")
     b, width = block_table.shape
-    _need(width <= 1 or block_table.stride(1) == 1,
-          "block_table: rows have to be contiguous")
-    _need(width * block < (1 << 31) - 4096,
-          "block_table: a sequence has room for 2^31 - 4096 slots at most")
-    _index("seq_lens", seq_lens, (b,), k_pool.device)
-    return n, block, kvh, d, b, width * block
-
-
-def _fields(k_pool, v_pool, block_table, seq_lens):
-    n, block, kvh, d = k_pool.shape
-    return [k_pool.data_ptr(), v_pool.data_ptr(), *k_pool.stride()[:3],
-            *v_pool.stride()[:3], n, block, kvh, d,
-            int(k_pool.dtype == torch.float16), block_table.data_ptr(),
-            int(block_table.dtype == torch.int64), block_table.stride(0),
-            block_table.shape[1], seq_lens.data_ptr(),
-            int(seq_lens.dtype == torch.int64), block_table.shape[0]]
+    row, one = block_table.stride()
+    if one != 1 and width > 1:
+        _refuse("block_table: rows have to be contiguous")
+    if width * block >= (1 << 31) - 4096:
+        _refuse("block_table: fewer than 2^31 - 4096 slots a sequence")
+    _array("seq_lens", seq_lens, None, (b,), dev)
+    return [k, v, k0, k1, k2, v0, v1, v2, n, block, kvh, d, dtype == _FP16,
+            block_table.data_ptr(), block_table.dtype == _I64, row, width,
+            seq_lens.data_ptr(), seq_lens.dtype == _I64, b], \
+        (block, kvh, d, b, width * block)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -127,26 +150,20 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 
 
 def _is64(t: Optional[torch.Tensor]) -> int:
-    return int(t is not None and t.dtype == torch.int64)
+    return t is not None and t.dtype == _I64
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _grouped(qh: int, kvh: int):
-    _need(qh >= kvh and qh % kvh == 0,
-          f"q: {qh} heads are no multiple of the {kvh} key heads")
-
-
-def _score_args(scale, softcap, slopes, d, qh, device):
+def _score_args(scale, softcap, slopes, d, qh, kvh, dev):
+    if qh < kvh or qh % kvh:
+        _refuse(f"q: {qh} heads are no multiple of the {kvh} key heads")
     scale = d ** -0.5 if scale is None else float(scale)
     softcap = float(softcap)
-    _need(math.isfinite(scale), f"scale: finite, got {scale}")
-    _need(math.isfinite(softcap) and softcap >= 0,
-          f"softcap: finite and not negative, got {softcap}")
+    if not math.isfinite(scale):
+        _refuse(f"scale: finite, got {scale}")
+    if not 0.0 <= softcap < math.inf:
+        _refuse(f"softcap: finite and not negative, got {softcap}")
     if slopes is not None:
-        _plane("slopes", slopes, torch.float32, (qh,), device)
+        _array("slopes", slopes, _F32, (qh,), dev)
     return scale, softcap
 
 
@@ -177,39 +194,36 @@ def paged_append_op(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
     dropped. `key_pos` [B, kvh, room] int32, if given, gets the tokens'
     positions `pos` [T] at their slots.
     """
-    n, block, kvh, d, b, room = _cache(k_pool, v_pool, block_table, seq_lens)
-    dev = k_pool.device
-    _no_grad(k, v)
-    for name, t in (("k", k), ("v", v)):
-        _need(t.dim() == 3 and t.shape[1:] == (kvh, d),
-              f"{name}: [T, {kvh}, {d}], got {tuple(t.shape)}")
-        _need(t.dtype == k_pool.dtype,
-              f"{name}: the pools' {k_pool.dtype}, got {t.dtype}")
-        _need(t.device == dev, f"{name}: on {t.device}, not on {dev}")
-        _rows16(name, t)
+    fields, (block, kvh, d, b, room) = _cache(k_pool, v_pool, block_table,
+                                              seq_lens)
+    dev, dtype = k_pool.device, k_pool.dtype
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _no_backward()
     tokens = k.shape[0]
-    _need(v.shape[0] == tokens, "k and v: as many tokens each")
-    if cu_seqlens is None:
-        _need(tokens == b, f"k: one token for each of {b} sequences, got "
-                           f"{tokens}; packed tokens need cu_seqlens")
-    else:
-        _index("cu_seqlens", cu_seqlens, (b + 1,), dev)
-    _need((key_pos is None) == (pos is None),
-          "key_pos and pos: both or neither")
-    if key_pos is not None:
-        _plane("key_pos", key_pos, torch.int32, (b, kvh, room), dev)
-        _index("pos", pos, (tokens,), dev)
+    if k.shape != (tokens, kvh, d) or v.shape != k.shape:
+        _refuse(f"k: and v: [T, {kvh}, {d}], got {tuple(k.shape)} and "
+                f"{tuple(v.shape)}")
+    _heads("k", k, dtype, dev)
+    _heads("v", v, dtype, dev)
+    if cu_seqlens is not None:
+        _array("cu_seqlens", cu_seqlens, None, (b + 1,), dev)
+    elif tokens != b:
+        _refuse(f"k: one token for each of {b} sequences, got {tokens}; "
+                "packed tokens need cu_seqlens")
+    if key_pos is not None and pos is not None:
+        _array("key_pos", key_pos, _I32, (b, kvh, room), dev)
+        _array("pos", pos, None, (tokens,), dev)
+    elif key_pos is not pos:
+        _refuse("key_pos and pos: both or neither")
     if not tokens or not b:
         return
-    if k_pool.is_cuda:
-        with torch.cuda.device(dev):
-            _C().paged_append(
-                _fields(k_pool, v_pool, block_table, seq_lens),
-                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                v.stride(0), v.stride(1), tokens, _ptr(cu_seqlens),
-                _is64(cu_seqlens), _ptr(key_pos), _ptr(pos), _is64(pos),
-                _stream(dev))
+    if dev.type == "cuda":
+        _call("paged_append", dev, fields, k.data_ptr(), k.stride(0),
+              k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), tokens,
+              _ptr(cu_seqlens), _is64(cu_seqlens), _ptr(key_pos), _ptr(pos),
+              _is64(pos))
         return
+    n = k_pool.shape[0]
     for i in range(b):
         lo = i if cu_seqlens is None else max(int(cu_seqlens[i]), 0)
         hi = i + 1 if cu_seqlens is None else min(int(cu_seqlens[i + 1]),
@@ -259,55 +273,54 @@ def paged_decode_op(q: torch.Tensor, k_pool: torch.Tensor,
     the sum of exponentials [B, qh] fp32 and the weights. A sequence that
     sees no key gets zeros and -inf.
     """
-    n, block, kvh, d, b, room = _cache(k_pool, v_pool, block_table, seq_lens)
+    fields, (block, kvh, d, b, room) = _cache(k_pool, v_pool, block_table,
+                                              seq_lens)
     dev = k_pool.device
-    _no_grad(q, slopes, mass)
-    _need(q.dim() == 3 and q.shape[0] == b and q.shape[2] == d,
-          f"q: [{b}, qh, {d}], got {tuple(q.shape)}")
-    _need(q.dtype == k_pool.dtype,
-          f"q: the pools' {k_pool.dtype}, got {q.dtype}")
-    _need(q.device == dev, f"q: on {q.device}, not on {dev}")
-    _need(d in (64, 128), f"q: d of 64 or 128, got {d}")
+    if torch.is_grad_enabled() and (
+            q.requires_grad or mass is not None and mass.requires_grad
+            or slopes is not None and slopes.requires_grad):
+        _no_backward()
+    if q.dim() != 3 or q.shape[0] != b or q.shape[2] != d:
+        _refuse(f"q: [{b}, qh, {d}], got {tuple(q.shape)}")
     qh = q.shape[1]
-    _grouped(qh, kvh)
-    _rows16("q", q)
-    scale, softcap = _score_args(scale, softcap, slopes, d, qh, dev)
-    _need((key_pos is None) == (q_pos is None),
-          "key_pos and q_pos: both or neither")
-    if key_pos is not None:
-        _plane("key_pos", key_pos, torch.int32, (b, kvh, room), dev)
-        _index("q_pos", q_pos, (b,), dev)
-    if mass is None:
-        _need(mass_out is None, "mass_out: needs mass")
-    else:
-        _plane("mass", mass, torch.float32, (b, kvh, room), dev)
+    if d != 128 and d != 64:
+        _refuse(f"q: d of 64 or 128, got {d}")
+    _heads("q", q, k_pool.dtype, dev)
+    scale, softcap = _score_args(scale, softcap, slopes, d, qh, kvh, dev)
+    if key_pos is not None and q_pos is not None:
+        _array("key_pos", key_pos, _I32, (b, kvh, room), dev)
+        _array("q_pos", q_pos, None, (b,), dev)
+    elif key_pos is not q_pos:
+        _refuse("key_pos and q_pos: both or neither")
+    if mass is not None:
+        _array("mass", mass, _F32, (b, kvh, room), dev)
         if mass_out is None:
             mass_out = torch.empty_like(mass)
         else:
-            _plane("mass_out", mass_out, torch.float32, (b, kvh, room), dev)
-            _need(mass_out.data_ptr() == mass.data_ptr()
-                  or not _overlap(mass, mass_out),
-                  "mass_out: mass itself, or apart from it")
-    out = torch.empty(b, qh, d, dtype=q.dtype, device=dev)
-    lse = torch.empty(b, qh, dtype=torch.float32, device=dev)
-    if b and k_pool.is_cuda:
-        with torch.cuda.device(dev):
-            ws = torch.empty(
-                _C().paged_decode_workspace(b, qh, kvh, d, room,
-                                            mass is not None),
-                dtype=torch.uint8, device=dev)
-            _C().paged_decode(
-                _fields(k_pool, v_pool, block_table, seq_lens),
-                q.data_ptr(), q.stride(0), q.stride(1), qh, scale, softcap,
-                _ptr(slopes), _ptr(key_pos), _ptr(q_pos), _is64(q_pos),
-                out.data_ptr(), lse.data_ptr(), _ptr(mass), _ptr(mass_out),
-                ws.data_ptr(), _stream(dev))
+            _array("mass_out", mass_out, _F32, (b, kvh, room), dev)
+            if mass_out.data_ptr() != mass.data_ptr() \
+                    and _overlap(mass, mass_out):
+                _refuse("mass_out: mass itself, or apart from it")
+    elif mass_out is not None:
+        _refuse("mass_out: needs mass")
+    cuda = dev.type == "cuda"
+    out = torch.empty((b, qh, d), dtype=q.dtype, device=dev)
+    lse = torch.empty((b, qh), dtype=_F32, device=dev) \
+        if return_lse or not cuda else None
+    if b and cuda:
+        ws = torch.empty(_native().paged_decode_workspace(
+            b, qh, kvh, d, room, mass is not None), dtype=torch.uint8,
+            device=dev)
+        _call("paged_decode", dev, fields, q.data_ptr(), q.stride(0),
+              q.stride(1), qh, scale, softcap, _ptr(slopes), _ptr(key_pos),
+              _ptr(q_pos), _is64(q_pos), out.data_ptr(), _ptr(lse),
+              _ptr(mass), _ptr(mass_out), ws.data_ptr())
     elif b:
         _decode_cpu(q, k_pool, v_pool, block_table, seq_lens, scale, softcap,
                     slopes, key_pos, q_pos, mass, mass_out, out, lse)
-    got = [out] + ([lse] if return_lse else []) \
-        + ([mass_out] if mass is not None else [])
-    return got[0] if len(got) == 1 else tuple(got)
+    if mass is not None:
+        return (out, lse, mass_out) if return_lse else (out, mass_out)
+    return (out, lse) if return_lse else out
 
 
 def _weights_cpu(s: torch.Tensor):
@@ -369,45 +382,45 @@ def kv_evict_op(k_pool: torch.Tensor, v_pool: torch.Tensor,
     be the inputs themselves. A page is moved by the one sequence that holds
     it: pages that sequences share must not be evicted from.
     """
-    n, block, kvh, d, b, room = _cache(k_pool, v_pool, block_table, seq_lens)
+    fields, (block, kvh, d, b, room) = _cache(k_pool, v_pool, block_table,
+                                              seq_lens)
     dev = k_pool.device
-    _plane("mass", mass, torch.float32, (b, kvh, room), dev)
-    _plane("key_pos", key_pos, torch.int32, (b, kvh, room), dev)
-    _no_grad(mass)
+    if mass.requires_grad and torch.is_grad_enabled():
+        _no_backward()
+    _array("mass", mass, _F32, (b, kvh, room), dev)
+    _array("key_pos", key_pos, _I32, (b, kvh, room), dev)
     budget, recent = int(budget), int(recent)
-    _need(1 <= budget < 1 << 31, f"budget: at least 1, got {budget}")
-    _need(0 <= recent <= budget,
-          f"recent: from 0 to the budget of {budget}, got {recent}")
+    if not 1 <= budget < 1 << 31:
+        _refuse(f"budget: at least 1, got {budget}")
+    if not 0 <= recent <= budget:
+        _refuse(f"recent: from 0 to the budget of {budget}, got {recent}")
     if out is None:
         out = (torch.empty_like(seq_lens), torch.empty_like(mass),
                torch.empty_like(key_pos))
     else:
-        _need(len(out) == 3, "out: (seq_lens, mass, key_pos)")
-        _plane("out[0]", out[0], seq_lens.dtype, (b,), dev)
-        _plane("out[1]", out[1], torch.float32, (b, kvh, room), dev)
-        _plane("out[2]", out[2], torch.int32, (b, kvh, room), dev)
-        for new, old in zip(out, (seq_lens, mass, key_pos)):
-            _need(new.data_ptr() == old.data_ptr()
-                  or not _overlap(new, old),
-                  "out: the inputs themselves, or apart from them")
+        out = tuple(out)
+        if len(out) != 3:
+            _refuse("out: (seq_lens, mass, key_pos)")
+        _array("out[0]", out[0], seq_lens.dtype, (b,), dev)
+        _array("out[1]", out[1], _F32, (b, kvh, room), dev)
+        _array("out[2]", out[2], _I32, (b, kvh, room), dev)
         for i, x in enumerate(out):
             for j, y in enumerate((seq_lens, mass, key_pos)):
-                _need(i == j or not _overlap(x, y),
-                      "out: not over another input")
-            for y in out[:i]:
-                _need(not _overlap(x, y), "out: apart from each other")
+                if (i != j or x.data_ptr() != y.data_ptr()) \
+                        and _overlap(x, y):
+                    _refuse("out: the inputs themselves, or apart from them")
+            if any(_overlap(x, y) for y in out[:i]):
+                _refuse("out: apart from each other")
     if not b:
         return out
-    if k_pool.is_cuda:
-        with torch.cuda.device(dev):
-            ws = torch.empty(
-                _C().kv_evict_workspace(b, kvh, room, budget),
-                dtype=torch.uint8, device=dev)
-            _C().kv_evict(_fields(k_pool, v_pool, block_table, seq_lens),
-                          mass.data_ptr(), key_pos.data_ptr(), budget,
-                          recent, out[1].data_ptr(), out[2].data_ptr(),
-                          out[0].data_ptr(), ws.data_ptr(), _stream(dev))
+    if dev.type == "cuda":
+        ws = torch.empty(_native().kv_evict_workspace(b, kvh, room, budget),
+                         dtype=torch.uint8, device=dev)
+        _call("kv_evict", dev, fields, mass.data_ptr(), key_pos.data_ptr(),
+              budget, recent, out[1].data_ptr(), out[2].data_ptr(),
+              out[0].data_ptr(), ws.data_ptr())
         return out
+    n = k_pool.shape[0]
     new_lens, new_mass = seq_lens.clone(), mass.clone()
     new_pos = key_pos.clone()
     for i in range(b):
@@ -468,60 +481,64 @@ def flash_prefill_packed_op(q: torch.Tensor, k: torch.Tensor,
     Keys and values of rows that a document's mask hides from part of its
     queries have to be finite.
     """
-    dev = q.device
-    _need(q.dim() == 3 and k.dim() == 3,
-          "q and k: [tokens, heads, d]")
-    _need(q.dtype in _HALF, f"q: bfloat16 or float16, got {q.dtype}")
+    dev, dtype = q.device, q.dtype
+    if q.dim() != 3 or k.dim() != 3:
+        _refuse("q and k: [tokens, heads, d]")
+    if dtype != _BF16 and dtype != _FP16:
+        _refuse(f"q: bfloat16 or float16, got {dtype}")
     rows, qh, d = q.shape
-    keys, kvh = k.shape[:2]
-    _need(d in (64, 128), f"q: d of 64 or 128, got {d}")
-    _need(kvh >= 1 and k.shape[2] == d, f"k: [Tk, kvh, {d}], got "
-                                        f"{tuple(k.shape)}")
-    _need(v.shape == k.shape, "v: of k's shape")
-    for name, t in (("k", k), ("v", v)):
-        _need(t.dtype == q.dtype, f"{name}: q's {q.dtype}, got {t.dtype}")
-        _need(t.device == dev, f"{name}: on {t.device}, not on {dev}")
-    _grouped(qh, kvh)
-    _no_grad(q, k, v, slopes)
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _rows16(name, t)
-        _need(t.shape[0] < 1 << 31, f"{name}: 2^31 rows at most")
-    _need(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1,
-          "cu_seqlens: [documents + 1]")
-    docs = cu_seqlens.numel() - 1
-    _index("cu_seqlens", cu_seqlens, (docs + 1,), dev)
-    if cu_seqlens_k is None:
-        _need(keys == rows, "k: as many rows as q, or cu_seqlens_k")
+    keys, kvh, dk = k.shape
+    if d != 128 and d != 64:
+        _refuse(f"q: d of 64 or 128, got {d}")
+    if kvh < 1 or dk != d:
+        _refuse(f"k: [Tk, kvh, {d}], got {tuple(k.shape)}")
+    if v.shape != k.shape:
+        _refuse("v: of k's shape")
+    if rows >= 1 << 31 or keys >= 1 << 31:
+        _refuse("q and k: fewer than 2^31 rows")
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or v.requires_grad
+            or slopes is not None and slopes.requires_grad):
+        _no_backward()
+    _heads("q", q, dtype, dev)
+    _heads("k", k, dtype, dev)
+    _heads("v", v, dtype, dev)
+    scale, softcap = _score_args(scale, softcap, slopes, d, qh, kvh, dev)
+    if cu_seqlens.dim() != 1 or not cu_seqlens.shape[0]:
+        _refuse("cu_seqlens: [documents + 1]")
+    docs = cu_seqlens.shape[0] - 1
+    _array("cu_seqlens", cu_seqlens, None, (docs + 1,), dev)
+    if cu_seqlens_k is not None:
+        _array("cu_seqlens_k", cu_seqlens_k, None, (docs + 1,), dev)
+    elif keys != rows:
+        _refuse("k: as many rows as q, or cu_seqlens_k")
+    else:
         cu_seqlens_k = cu_seqlens
-    else:
-        _index("cu_seqlens_k", cu_seqlens_k, (docs + 1,), dev)
     if prefix_lens is not None:
-        _need(causal, "prefix_lens: without causal every key is seen")
-        _index("prefix_lens", prefix_lens, (docs,), dev)
-    scale, softcap = _score_args(scale, softcap, slopes, d, qh, dev)
+        if not causal:
+            _refuse("prefix_lens: without causal every key is seen")
+        _array("prefix_lens", prefix_lens, None, (docs,), dev)
     clear = out is None
-    if out is None:
-        out = torch.empty(rows, qh, d, dtype=q.dtype, device=dev)
+    if clear:
+        out = torch.empty((rows, qh, d), dtype=dtype, device=dev)
     else:
-        _need(out.shape == q.shape and out.dtype == q.dtype
-              and out.device == dev, "out: of q's shape, type and device")
-        _rows16("out", out)
-        _need(not any(_overlap(out, t) for t in (q, k, v)),
-              "out: apart from q, k and v")
-    lse = torch.empty(rows, qh, dtype=torch.float32, device=dev) \
+        if out.shape != q.shape:
+            _refuse(f"out: of q's shape, got {tuple(out.shape)}")
+        _heads("out", out, dtype, dev)
+        if _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
+            _refuse("out: apart from q, k and v")
+    lse = torch.empty((rows, qh), dtype=_F32, device=dev) \
         if return_lse else None
-    if rows and q.is_cuda:
-        with torch.cuda.device(dev):
-            _C().packed_prefill(
-                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
-                k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                v.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                _ptr(lse), rows, keys, qh, kvh, d,
-                int(q.dtype == torch.float16), docs, cu_seqlens.data_ptr(),
-                _is64(cu_seqlens), cu_seqlens_k.data_ptr(),
-                _is64(cu_seqlens_k), _ptr(prefix_lens), _is64(prefix_lens),
-                int(causal), int(clear), scale, softcap, _ptr(slopes),
-                _stream(dev))
+    if rows and dev.type == "cuda":
+        _call("packed_prefill", dev, q.data_ptr(), q.stride(0), q.stride(1),
+              k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+              v.stride(0), v.stride(1), out.data_ptr(), out.stride(0),
+              out.stride(1), _ptr(lse), rows, keys, qh, kvh, d,
+              dtype == _FP16, docs, cu_seqlens.data_ptr(),
+              cu_seqlens.dtype == _I64, cu_seqlens_k.data_ptr(),
+              cu_seqlens_k.dtype == _I64, _ptr(prefix_lens),
+              _is64(prefix_lens), causal, clear, scale, softcap,
+              _ptr(slopes))
     elif rows:
         if clear:
             out.zero_()
