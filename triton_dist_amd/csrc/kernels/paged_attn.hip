@@ -19,12 +19,37 @@ void launched(const char *what) {
     throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
 }
 
+// Of all lanes, to all lanes: lane i takes from lanes 1, 2, 4 and 8 before it
+// in its row of 16, then rows 1 and 3 from the row before, then 2 and 3 from
+// lane 31, which leaves the whole in lane 63.
+#define TD_WAVE_STEPS(X) \
+  X(0x111, 0xf) X(0x112, 0xf) X(0x114, 0xf) X(0x118, 0xf) X(0x142, 0xa) \
+  X(0x143, 0xc)
 TD_DEV float wave_max(float x) {
-  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return x;
+#define TD_STEP(ctrl, rows)                                                 \
+  x = fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(                 \
+                   __float_as_uint(x), __float_as_uint(x), ctrl, rows, 0xf, \
+                   false)));
+  TD_WAVE_STEPS(TD_STEP)
+#undef TD_STEP
+  return __uint_as_float(
+      __builtin_amdgcn_readlane(__float_as_uint(x), 63));
 }
 TD_DEV float wave_sum(float x) {
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+#define TD_STEP(ctrl, rows)                                             \
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(                     \
+      0, __float_as_uint(x), ctrl, rows, 0xf, true));
+  TD_WAVE_STEPS(TD_STEP)
+#undef TD_STEP
+  return __uint_as_float(
+      __builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+// Sums over the lanes up to and with this one.
+TD_DEV int wave_scan(int x) {
+#define TD_STEP(ctrl, rows) \
+  x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, true);
+  TD_WAVE_STEPS(TD_STEP)
+#undef TD_STEP
   return x;
 }
 
@@ -91,7 +116,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 32;              // keys of a wave's step
 constexpr int kStep = 4 * kTile;       // keys of a workgroup's step
-constexpr int kSlots = 768;            // workgroups that the card holds
+constexpr int kSlots = 1024;            // workgroups that the card holds
 
 template <typename T> using vec8 = __attribute__((ext_vector_type(8))) T;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
@@ -119,65 +144,91 @@ TD_DEV void wave_fence() {
 struct Chunk {
   int b, len;        // sequence and its length
   int first, count;  // this chunk's number among the sequence's, how many
-  int id;            // over the whole batch
   int steps;         // of kStep keys, a chunk's length
 };
 
-// The chunk `id` of the batch, or (id < 0) sequence `seq`'s first one. A
-// sequence has one chunk at least. Every wave finds its own.
-TD_DEV bool find_chunk(const PagedArgs &c, int target, int least, int id,
-                       int seq, Chunk &out) {
-  const int lane = threadIdx.x & 63;
-  long total = 0;
-  int len = 0;
-  for (int base = 0; base < c.batch; base += 64) {
-    len = base + lane < c.batch ? c.len(base + lane) : 0;
-    int t = (len + kStep - 1) / kStep;
-    for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o);
-    total += t;
+// A sequence's first chunk has the sequence's number, so that finding it
+// takes nothing; the further ones are numbered behind those, sequence by
+// sequence, and are found by a sum over the batch. All of a workgroup of 256
+// threads calls these.
+struct Cut {
+  int steps;  // a chunk's length
+  int each;   // sequences that a thread sums over
+};
+// How long chunks are, from the lengths of the whole batch.
+TD_DEV Cut find_cut(const PagedArgs &c, int target, int least, int *lds) {
+  const int tid = threadIdx.x;
+  Cut cut;
+  cut.each = (c.batch + 255) / 256;
+  int sum = 0;
+  for (int i = tid * cut.each; i < min((tid + 1) * cut.each, c.batch); ++i)
+    sum += (c.len(i) + kStep - 1) / kStep;
+  sum = wave_scan(sum);
+  __syncthreads();
+  if ((tid & 63) == 63) lds[tid >> 6] = sum;
+  __syncthreads();
+  const long total = (long)lds[0] + lds[1] + lds[2] + lds[3];
+  cut.steps = max(least, (int)((total + target - 1) / target));
+  return cut;
+}
+TD_DEV int chunks_of(int len, int steps) {
+  return max(1, ((len + kStep - 1) / kStep + steps - 1) / steps);
+}
+// The further chunks before this thread's sequences; `all` of the batch.
+TD_DEV int further_before(const PagedArgs &c, const Cut &cut, int *lds,
+                          int &all) {
+  const int tid = threadIdx.x;
+  int own = 0;
+  for (int i = tid * cut.each; i < min((tid + 1) * cut.each, c.batch); ++i)
+    own += chunks_of(c.len(i), cut.steps) - 1;
+  const int upto = wave_scan(own);
+  __syncthreads();
+  if ((tid & 63) == 63) lds[tid >> 6] = upto;
+  __syncthreads();
+  int before = upto - own;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < tid >> 6) before += lds[i];
+    all += lds[i];
   }
-  total = __builtin_amdgcn_readfirstlane((int)min(total, 0x7fffffffL));
-  out.steps = max(least, (int)((total + target - 1) / target));
-  int before = 0;
-  for (int base = 0; base < c.batch; base += 64) {
-    if (c.batch > 64) len = base + lane < c.batch ? c.len(base + lane) : 0;
-    const int t = (len + kStep - 1) / kStep;
-    const int n = base + lane < c.batch
-                      ? max(1, (t + out.steps - 1) / out.steps)
-                      : 0;
-    int upto = n;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o);
-      if (lane >= o) upto += x;
+  return before;
+}
+// The further chunk `at`; false where there are not so many.
+TD_DEV bool find_further(const PagedArgs &c, const Cut &cut, int at,
+                         int *lds, Chunk &out) {
+  int all;
+  int before = further_before(c, cut, lds, all);
+  if (at >= all) return false;
+  const int tid = threadIdx.x;
+  for (int i = tid * cut.each; i < min((tid + 1) * cut.each, c.batch); ++i) {
+    const int n = chunks_of(c.len(i), cut.steps) - 1;
+    if (at >= before && at < before + n) {
+      lds[4] = i;
+      lds[5] = at - before + 1;
     }
-    const bool here = id >= 0 ? before + upto > id : base + lane == seq;
-    const unsigned long long found = __ballot(here);
-    if (found) {
-      const int f = __builtin_ctzll(found);
-      out.b = base + f;
-      out.len = __builtin_amdgcn_readlane(len, f);
-      out.count = __builtin_amdgcn_readlane(n, f);
-      const int start = before + __builtin_amdgcn_readlane(upto, f) -
-                        out.count;
-      out.first = id >= 0 ? id - start : 0;
-      out.id = start + out.first;
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    before += n;
   }
-  return false;
+  __syncthreads();
+  out.b = lds[4];
+  out.first = lds[5];
+  out.len = c.len(out.b);
+  out.steps = cut.steps;
+  out.count = chunks_of(out.len, cut.steps);
+  return true;
 }
 
 // Where a call keeps what its kernels hand on.
 struct DecodeWork {
-  float *part;    // [chunks, qh, d]: a chunk's outputs
+  float *part;    // [chunks, qh, d]: outputs of one chunk among several
   float *sum;     // [chunks, qh]: log2 of a chunk's sum
+  int *plan;      // [batch, 2]: a sequence's chunks, its first further one
   float *logits;  // [batch, qh, room], in units of log2, where weights are
   int target, least, groups;
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 3) void k_paged_decode(PagedDecodeArgs a,
+__global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
                                                          DecodeWork w) {
   constexpr int kC = D / 32, kT = D / 16;  // pieces of a row, tiles of it
   constexpr int kRow = D + 16;   // of V in LDS: 8 rows take all 64 banks
@@ -186,12 +237,28 @@ __global__ __launch_bounds__(256, 3) void k_paged_decode(PagedDecodeArgs a,
   static_assert(16 * kORow * 4 <= kBytes, "outputs fit where V was");
   __shared__ __attribute__((aligned(16))) char lds[4][kBytes];
   __shared__ float lds_m[4][16], lds_l[4][16];
+  __shared__ int found[8];
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int n = lane & 15, qd = lane >> 4;
   const int per = a.c.kvh * w.groups;
-  Chunk ch;
-  if (!find_chunk(a.c, w.target, w.least, blockIdx.x / per, 0, ch)) return;
+  const int id = blockIdx.x / per;
+  Chunk ch{id, 0, 0, 1, w.least};
+  if (id >= a.c.batch) {
+    if (!find_further(a.c, find_cut(a.c, w.target, w.least, found),
+                      id - a.c.batch, found, ch))
+      return;
+  } else {
+    ch.len = a.c.len(id);
+    if (ch.len > w.least * kStep) {
+      ch.steps = find_cut(a.c, w.target, w.least, found).steps;
+      ch.count = chunks_of(ch.len, ch.steps);
+    }
+  }
+  if (tid == 0 && blockIdx.x % per == 0) {
+    if (ch.first == 0) w.plan[2 * ch.b] = ch.count;
+    if (ch.first == 1) w.plan[2 * ch.b + 1] = id;
+  }
   const int kh = blockIdx.x % per / w.groups;
   const int group = blockIdx.x % per % w.groups;
   const int g = a.qh / a.c.kvh;
@@ -222,6 +289,7 @@ __global__ __launch_bounds__(256, 3) void k_paged_decode(PagedDecodeArgs a,
   const T *kbase = (const T *)a.c.k + kh * a.c.k_head + qd * 8;
   const T *vbase = (const T *)a.c.v + kh * a.c.v_head + qd * 8;
   vec8<T> kf[2][kC], vf[2][kC];
+  int kp[2][4];    // positions of the loaded tile's keys 16 t + 4 qd + i
   int page[2];     // of the tile to load next
   bool ok[2];      // this lane's rows of the loaded tile are there
   auto look_up = [&](int base) {
@@ -242,6 +310,10 @@ __global__ __launch_bounds__(256, 3) void k_paged_decode(PagedDecodeArgs a,
 #pragma unroll
       for (int c = 0; c < kC; ++c)
         kf[t][c] = *(const vec8<T> *)(row + c * 32);
+      if (key_pos)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          kp[t][i] = key_pos[min(base + 16 * t + 4 * qd + i, k1 - 1)];
     }
   };
   auto load_v = [&](int base) {
@@ -274,6 +346,16 @@ __global__ __launch_bounds__(256, 3) void k_paged_decode(PagedDecodeArgs a,
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int c = 0; c < kC; ++c) s[t] = mfma16(kf[t][c], qf[c], s[t]);
+    float far[2][4];
+    if (a.s.slopes) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          far[t][i] = fabsf((float)(
+              key_pos ? q_at - kp[t][i]
+                      : q_at - (base + 16 * t + 4 * qd + i)));
+    }
     // which of the tile's 32 rows are there, seen by every lane
     const unsigned here = (unsigned)(__ballot(ok[0]) & 0xffff) |
                           (unsigned)(__ballot(ok[1]) & 0xffff) << 16;
@@ -313,13 +395,7 @@ __global__ __launch_bounds__(256, 3) void k_paged_decode(PagedDecodeArgs a,
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int slot = base + 16 * t + 4 * qd + i;
-          long far = slot;
-          if (key_pos) far = key_pos[min(slot, k1 - 1)];
-          far = q_at - far;
-          s[t][i] -= slope * (float)(far < 0 ? -far : far);
-        }
+        for (int i = 0; i < 4; ++i) s[t][i] -= slope * far[t][i];
     }
     if (here != 0xffffffffu) {
 #pragma unroll
@@ -403,74 +479,99 @@ __global__ __launch_bounds__(256, 3) void k_paged_decode(PagedDecodeArgs a,
     o *= sum == 0.f ? 0.f : 1.f / sum;
     const float lse = sum == 0.f ? -INFINITY
                                  : top + __builtin_amdgcn_logf(sum);
+    const long at = (long)id * a.qh + h0 + h;
     if (ch.count == 1) {
       T *to = (T *)a.out + ((long)b * a.qh + h0 + h) * D + c;
 #pragma unroll
       for (int x = 0; x < 4; ++x) to[x] = (T)o[x];
-      if (c == 0) a.lse[(long)b * a.qh + h0 + h] = lse * kLn2;
+      if (c == 0 && a.lse) a.lse[(long)b * a.qh + h0 + h] = lse * kLn2;
     } else {
-      const long at = (long)ch.id * a.qh + h0 + h;
       *(f32x4 *)(w.part + at * D + c) = o;
-      if (c == 0) w.sum[at] = lse;
     }
+    if (c == 0) w.sum[at] = lse;
   }
 }
 
-// Joins the chunks of a sequence's query head: a wave each.
+// Joins a sequence's chunks and hands out its weights: of the workgroups
+// (sequence, key head, z) the first ones join a query head each, and each
+// further one adds the weights of 1024 slots, from the logits that the first
+// kernel kept.
+constexpr int kSpan = 1024;
 template <typename T, int D>
-__global__ __launch_bounds__(64) void k_decode_join(PagedDecodeArgs a,
-                                                    DecodeWork w) {
-  Chunk ch;
-  const int h = blockIdx.y, lane = threadIdx.x;
-  find_chunk(a.c, w.target, w.least, -1, blockIdx.x, ch);
-  if (ch.count == 1) return;
-  const float *sum = w.sum + (long)ch.id * a.qh + h;
-  const float *part = w.part + ((long)ch.id * a.qh + h) * D + lane * (D / 64);
-  float top = -INFINITY;
-  for (int i = lane; i < ch.count; i += 64)
-    top = fmaxf(top, sum[(long)i * a.qh]);
-  top = wave_max(top);
-  const float safe = top == -INFINITY ? 0.f : top;
-  float total = 0.f, o[D / 64] = {};
-  for (int i = 0; i < ch.count; ++i) {
-    const float r = __builtin_amdgcn_exp2f(sum[(long)i * a.qh] - safe);
-    total += r;
-#pragma unroll
-    for (int x = 0; x < D / 64; ++x)
-      o[x] += r * part[(long)i * a.qh * D + x];
-  }
-  const float f = total == 0.f ? 0.f : 1.f / total;
-  T *out = (T *)a.out + ((long)ch.b * a.qh + h) * D + lane * (D / 64);
-#pragma unroll
-  for (int x = 0; x < D / 64; ++x) out[x] = (T)(o[x] * f);
-  if (lane == 0)
-    a.lse[(long)ch.b * a.qh + h] =
-        total == 0.f ? -INFINITY
-                     : (top + __builtin_amdgcn_logf(total)) * kLn2;
-}
-
-// The weights that the query heads of a key head gave each slot, from the
-// logits that the first kernel kept.
-__global__ __launch_bounds__(256) void k_decode_mass(PagedDecodeArgs a,
-                                                     DecodeWork w) {
-  const int b = blockIdx.y, kh = blockIdx.z, g = a.qh / a.c.kvh;
-  const int slot = blockIdx.x * 256 + threadIdx.x, room = a.c.room();
-  if (slot >= room) return;
-  const long at = ((long)b * a.c.kvh + kh) * room + slot;
-  float m = 0.f;
-  if (slot < a.c.len(b)) {
-    m = a.mass[at];
-    const float *s = w.logits + ((long)b * a.qh + kh * g) * room + slot;
-    const float *lse = a.lse + (long)b * a.qh + kh * g;
+__global__ __launch_bounds__(256) void k_decode_finish(PagedDecodeArgs a,
+                                                       DecodeWork w) {
+  __shared__ float lds_lse[4], lds_o[4][D];
+  const int b = blockIdx.x, kh = blockIdx.y, z = blockIdx.z;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int g = a.qh / a.c.kvh, room = a.c.room();
+  const int count = w.plan[2 * b], more = w.plan[2 * b + 1];
+  auto row = [&](int i, int h) {  // a chunk's outputs of a query head
+    return (long)(i ? more + i - 1 : b) * a.qh + h;
+  };
+  auto lse_of = [&](int h, float &top) {  // the whole wave
+    top = -INFINITY;
+    for (int i = lane; i < count; i += 64)
+      top = fmaxf(top, w.sum[row(i, h)]);
+    top = wave_max(top);
+    const float safe = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
-    for (int i = 0; i < g; ++i) {
-      const float x = lse[i];
-      if (x != -INFINITY)
-        sum += __builtin_amdgcn_exp2f(s[(long)i * room] - x * kLog2e);
+    for (int i = lane; i < count; i += 64)
+      sum += __builtin_amdgcn_exp2f(w.sum[row(i, h)] - safe);
+    sum = wave_sum(sum);
+    return sum == 0.f ? -INFINITY : safe + __builtin_amdgcn_logf(sum);
+  };
+  if (z < g) {
+    if (count == 1) return;
+    const int h = kh * g + z;
+    float top;
+    const float lse = lse_of(h, top);
+    const float safe = lse == -INFINITY ? 0.f : lse;
+    float o[D / 64] = {};
+#pragma unroll 4
+    for (int i = wave; i < count; i += 4) {
+      const long at = row(i, h);
+      const float r = __builtin_amdgcn_exp2f(w.sum[at] - safe);
+#pragma unroll
+      for (int y = 0; y < D / 64; ++y)
+        o[y] += r * w.part[at * D + lane * (D / 64) + y];
     }
-    m += sum;
+#pragma unroll
+    for (int y = 0; y < D / 64; ++y) lds_o[wave][lane * (D / 64) + y] = o[y];
+    __syncthreads();
+    if (tid < D)
+      ((T *)a.out)[((long)b * a.qh + h) * D + tid] =
+          (T)(lds_o[0][tid] + lds_o[1][tid] + lds_o[2][tid] + lds_o[3][tid]);
+    if (tid == 0 && a.lse) a.lse[(long)b * a.qh + h] = lse * kLn2;
+    return;
   }
-  a.mass_out[at] = m;
+  const int len = a.c.len(b);
+  const long plane = ((long)b * a.c.kvh + kh) * room;
+  const int from = (z - g) * kSpan + tid;
+  float sum[kSpan / 256] = {};
+  if ((z - g) * kSpan < len)
+    for (int x = 0; x < g; x += 4) {
+      __syncthreads();
+      float top, lse = -INFINITY;
+      if (x + wave < g) lse = lse_of(kh * g + x + wave, top);
+      if (lane == 0) lds_lse[wave] = lse;
+      __syncthreads();
+      for (int y = 0; y < min(4, g - x); ++y) {
+        const float total = lds_lse[y];
+        if (total == -INFINITY) continue;
+        const float *s = w.logits + ((long)b * a.qh + kh * g + x + y) * room;
+#pragma unroll
+        for (int i = 0; i < kSpan / 256; ++i)
+          if (from + i * 256 < len)
+            sum[i] += __builtin_amdgcn_exp2f(s[from + i * 256] - total);
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < kSpan / 256; ++i) {
+    const int slot = from + i * 256;
+    if (slot < room)
+      a.mass_out[plane + slot] = slot < len ? a.mass[plane + slot] + sum[i]
+                                            : 0.f;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -632,8 +733,7 @@ size_t paged_decode_workspace(int batch, int qh, int kvh, int d, long room,
                               bool mass) {
   const DecodeWork w = decode_work(batch, qh, kvh);
   const size_t chunks = (size_t)w.target + batch;
-  return (chunks * qh * (d + 1) + (size_t)batch * qh +
-          (mass ? (size_t)batch * qh * room : 0)) *
+  return (chunks * qh * (d + 1) + 2 * (size_t)batch + (mass ? (size_t)batch * qh * room : 0)) *
          sizeof(float);
 }
 
@@ -645,34 +745,31 @@ static void decode(const PagedDecodeArgs &a, const DecodeWork &w,
     throw std::runtime_error("paged_decode: too many sequences and heads");
   k_paged_decode<T, D><<<dim3((unsigned)blocks), 256, 0, stream>>>(a, w);
   launched("paged_decode");
-  if (a.c.room() > w.least * kStep) {  // else no sequence has two chunks
-    k_decode_join<T, D><<<dim3(a.c.batch, a.qh), 64, 0, stream>>>(a, w);
+  // nothing to join where no sequence can have two chunks
+  const int spans = a.mass ? (a.c.room() + kSpan - 1) / kSpan : 0;
+  if (spans || a.c.room() > w.least * kStep) {
+    const dim3 finish(a.c.batch, a.c.kvh, a.qh / a.c.kvh + spans);
+    k_decode_finish<T, D><<<finish, 256, 0, stream>>>(a, w);
     launched("paged_decode");
   }
 }
 
-void launch_paged_decode(const PagedDecodeArgs &args, hipStream_t stream) {
-  PagedDecodeArgs a = args;
+void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
   if (!a.c.batch) return;
-  if (a.c.batch > 65535 || a.c.kvh > 65535)
-    throw std::runtime_error("paged_decode: 65535 sequences and heads at most");
+  if (a.c.kvh > 65535 || a.qh / a.c.kvh + a.c.room() / kSpan > 65534)
+    throw std::runtime_error("paged_decode: 65535 key heads and 2^25 slots of "
+                             "a sequence at most");
   DecodeWork w = decode_work(a.c.batch, a.qh, a.c.kvh);
   w.part = (float *)a.ws;
   w.sum = w.part + ((size_t)w.target + a.c.batch) * a.qh * a.c.d;
-  float *lse = w.sum + ((size_t)w.target + a.c.batch) * a.qh;
-  if (!a.lse) a.lse = lse;
-  w.logits = a.mass ? lse + (size_t)a.c.batch * a.qh : nullptr;
+  w.plan = (int *)(w.sum + ((size_t)w.target + a.c.batch) * a.qh);
+  w.logits = a.mass ? (float *)(w.plan + 2 * (size_t)a.c.batch) : nullptr;
   if (a.c.is_fp16)
     a.c.d == 64 ? decode<_Float16, 64>(a, w, stream)
                 : decode<_Float16, 128>(a, w, stream);
   else
     a.c.d == 64 ? decode<bf16, 64>(a, w, stream)
                 : decode<bf16, 128>(a, w, stream);
-  if (a.mass && a.c.room()) {
-    const dim3 grid((a.c.room() + 255) / 256, a.c.batch, a.c.kvh);
-    k_decode_mass<<<grid, 256, 0, stream>>>(a, w);
-    launched("paged_decode");
-  }
 }
 
 size_t kv_evict_workspace(int batch, int kvh, long room, int budget) {
