@@ -116,11 +116,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 32;              // keys of a wave's step
 constexpr int kStep = 4 * kTile;       // keys of a workgroup's step
-constexpr int kSlots = 1024;            // workgroups that the card holds
+constexpr int kSlots = 512;            // workgroups that the card holds
+constexpr int kFew = 6;                // steps that a workgroup starts for
 
 template <typename T> using vec8 = __attribute__((ext_vector_type(8))) T;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
+// at any float's address
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 TD_DEV f32x4 mfma16(vec8<bf16> a, vec8<bf16> b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -168,7 +172,13 @@ TD_DEV Cut find_cut(const PagedArgs &c, int target, int least, int *lds) {
   if ((tid & 63) == 63) lds[tid >> 6] = sum;
   __syncthreads();
   const long total = (long)lds[0] + lds[1] + lds[2] + lds[3];
-  cut.steps = max(least, (int)((total + target - 1) / target));
+  // One chunk a workgroup that the card holds, where that makes short ones
+  // (starting takes as long as a few steps); else two, which even out what
+  // ragged sequences leave over.
+  cut.steps = (int)((total + target - 1) / target);
+  if (cut.steps > kFew) cut.steps = (int)((total + 2 * target - 1) /
+                                          (2 * target));
+  cut.steps = max(least, cut.steps);
   return cut;
 }
 TD_DEV int chunks_of(int len, int steps) {
@@ -289,7 +299,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
   const T *kbase = (const T *)a.c.k + kh * a.c.k_head + qd * 8;
   const T *vbase = (const T *)a.c.v + kh * a.c.v_head + qd * 8;
   vec8<T> kf[2][kC], vf[2][kC];
-  int kp[2][4];    // positions of the loaded tile's keys 16 t + 4 qd + i
+  i32x4_any kp[2];  // positions of the loaded tile's keys 16 t + 4 qd + i
   int page[2];     // of the tile to load next
   bool ok[2];      // this lane's rows of the loaded tile are there
   auto look_up = [&](int base) {
@@ -310,10 +320,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
 #pragma unroll
       for (int c = 0; c < kC; ++c)
         kf[t][c] = *(const vec8<T> *)(row + c * 32);
-      if (key_pos)
+      if (key_pos) {
+        const int slot = base + 16 * t + 4 * qd;
+        if (slot + 4 <= k1) {
+          kp[t] = *(const i32x4_any *)(key_pos + slot);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          kp[t][i] = key_pos[min(base + 16 * t + 4 * qd + i, k1 - 1)];
+          for (int i = 0; i < 4; ++i)
+            kp[t][i] = key_pos[min(slot + i, k1 - 1)];
+        }
+      }
     }
   };
   auto load_v = [&](int base) {
@@ -405,13 +421,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
           if (!(here >> (16 * t + 4 * qd + i) & 1)) s[t][i] = -INFINITY;
     }
     if (w.logits && n < heads) {
-      float *to = w.logits + ((long)b * a.qh + h0 + n) * a.c.room() + base;
+      float *to = w.logits + ((long)b * a.qh + h0 + n) * a.c.room() + base +
+                  4 * qd;
+      if (base + kTile <= k1) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) *(f32x4_any *)(to + 16 * t) = s[t];
+      } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (base + 16 * t + 4 * qd + i < k1) to[16 * t + 4 * qd + i] =
-              s[t][i];
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (base + 16 * t + 4 * qd + i < k1) to[16 * t + i] = s[t][i];
+      }
     }
     float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]),
                             fmaxf(s[0][2], s[0][3])),
@@ -550,19 +571,27 @@ __global__ __launch_bounds__(256) void k_decode_finish(PagedDecodeArgs a,
   float sum[kSpan / 256] = {};
   if ((z - g) * kSpan < len)
     for (int x = 0; x < g; x += 4) {
+      float s[4][kSpan / 256];
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int i = 0; i < kSpan / 256; ++i)
+          s[y][i] = x + y < g && from + i * 256 < len
+                        ? w.logits[((long)b * a.qh + kh * g + x + y) * room +
+                                   from + i * 256]
+                        : -INFINITY;
       __syncthreads();
       float top, lse = -INFINITY;
       if (x + wave < g) lse = lse_of(kh * g + x + wave, top);
       if (lane == 0) lds_lse[wave] = lse;
       __syncthreads();
-      for (int y = 0; y < min(4, g - x); ++y) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
         const float total = lds_lse[y];
-        if (total == -INFINITY) continue;
-        const float *s = w.logits + ((long)b * a.qh + kh * g + x + y) * room;
+        if (total == -INFINITY) continue;  // also a head that is not there
 #pragma unroll
         for (int i = 0; i < kSpan / 256; ++i)
-          if (from + i * 256 < len)
-            sum[i] += __builtin_amdgcn_exp2f(s[from + i * 256] - total);
+          sum[i] += __builtin_amdgcn_exp2f(s[y][i] - total);
       }
     }
 #pragma unroll
@@ -732,7 +761,7 @@ static DecodeWork decode_work(int batch, int qh, int kvh) {
 size_t paged_decode_workspace(int batch, int qh, int kvh, int d, long room,
                               bool mass) {
   const DecodeWork w = decode_work(batch, qh, kvh);
-  const size_t chunks = (size_t)w.target + batch;
+  const size_t chunks = 2 * (size_t)w.target + batch;
   return (chunks * qh * (d + 1) + 2 * (size_t)batch + (mass ? (size_t)batch * qh * room : 0)) *
          sizeof(float);
 }
@@ -740,7 +769,7 @@ size_t paged_decode_workspace(int batch, int qh, int kvh, int d, long room,
 template <typename T, int D>
 static void decode(const PagedDecodeArgs &a, const DecodeWork &w,
                    hipStream_t stream) {
-  const long blocks = ((long)w.target + a.c.batch) * a.c.kvh * w.groups;
+  const long blocks = (2 * (long)w.target + a.c.batch) * a.c.kvh * w.groups;
   if (blocks > 0x7fffffffL)
     throw std::runtime_error("paged_decode: too many sequences and heads");
   k_paged_decode<T, D><<<dim3((unsigned)blocks), 256, 0, stream>>>(a, w);
@@ -761,8 +790,9 @@ void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
                              "a sequence at most");
   DecodeWork w = decode_work(a.c.batch, a.qh, a.c.kvh);
   w.part = (float *)a.ws;
-  w.sum = w.part + ((size_t)w.target + a.c.batch) * a.qh * a.c.d;
-  w.plan = (int *)(w.sum + ((size_t)w.target + a.c.batch) * a.qh);
+  const size_t chunks = 2 * (size_t)w.target + a.c.batch;
+  w.sum = w.part + chunks * a.qh * a.c.d;
+  w.plan = (int *)(w.sum + chunks * a.qh);
   w.logits = a.mass ? (float *)(w.plan + 2 * (size_t)a.c.batch) : nullptr;
   if (a.c.is_fp16)
     a.c.d == 64 ? decode<_Float16, 64>(a, w, stream)
