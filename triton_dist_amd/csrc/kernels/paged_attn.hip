@@ -605,9 +605,15 @@ __global__ __launch_bounds__(256) void k_decode_finish(PagedDecodeArgs a,
 
 // ---------------------------------------------------------------------------
 // evict
+//
+// Two launches: a workgroup per sequence and key head finds what stays, does
+// the bookkeeping and lists which row goes where; then all the card moves
+// rows. Bound by latency in the first (a dozen passes over registers with a
+// barrier each), by the rows' bytes in the second. Rows that stay below the
+// budget are not touched, so the steady state, one row over, moves one.
 // ---------------------------------------------------------------------------
 // Order of what stays: slots of the `recent` newest positions first, then
-// by weight, NaN above all as a sort has it. Unsigned compare.
+// by weight, NaN above all as a sort has it. Unsigned compare; never 0.
 TD_DEV unsigned rank_key(float mass, bool is_recent) {
   if (is_recent) return 0xFFFFFFFFu;
   if (mass != mass) return 0xFFFFFFFEu;
@@ -615,120 +621,241 @@ TD_DEV unsigned rank_key(float mass, bool is_recent) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// A workgroup per sequence and key head finds the kept slots and writes
-// which row goes where: the i-th free slot below the budget takes the i-th
-// kept row above it. ws: [batch, kvh] counts, then [batch, kvh, pairs, 2].
-__global__ __launch_bounds__(256) void k_evict_select(EvictArgs a,
-                                                      int pairs) {
-  __shared__ int red[256];
-  __shared__ unsigned pick;
-  __shared__ int need, off_hole, off_mover;
-  const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+constexpr int kEvict = 1024;              // threads, and slots of a pass
+constexpr int kEvictWaves = kEvict / 64;
+constexpr int kPairs = 64;                // rows that a workgroup moves
+
+// What goes where: the i-th free slot below the budget takes the i-th kept
+// row above it. ws: [batch, kvh] counts, then [batch, kvh, pairs] of these.
+struct Pair {
+  int to, from;
+};
+
+// R passes of slots are kept in registers as keys; longer sequences (MANY)
+// go by in parts of as many and are read again for each threshold.
+template <int R, bool MANY>
+__global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
+                                                         int pairs) {
+  __shared__ int lds_n[2][4][kEvictWaves];
+  __shared__ int lds_c[3][R][kEvictWaves];
+  const int b = blockIdx.x / a.c.kvh, h = blockIdx.x % a.c.kvh;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int room = a.c.room(), len = a.c.len(b);
+  const int keep = min(len, a.budget);
   const long row = ((long)b * a.c.kvh + h) * room;
   const float *mass = a.mass + row;
   const int *pos = a.key_pos + row;
-  int *count = (int *)a.ws + (long)b * a.c.kvh + h;
-  int *list = (int *)a.ws + (long)a.c.batch * a.c.kvh +
-              ((long)b * a.c.kvh + h) * pairs * 2;
-  const int keep = min(len, a.budget);
-  if (keep < len) {
-    int newest = INT_MIN;
-    for (int i = tid; i < len; i += 256) newest = max(newest, pos[i]);
-    red[tid] = newest;
-    __syncthreads();
-    if (tid == 0)
-      for (int i = 1; i < 256; ++i) newest = max(newest, red[i]);
-    if (tid == 0) red[0] = newest;
-    __syncthreads();
-    const long since = (long)red[0] - a.recent;
-    // the keep-th largest key, a bit at a time from the top
-    unsigned t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned with = t | 1u << bit;
-      int n = 0;
-      for (int i = tid; i < len; i += 256)
-        n += rank_key(mass[i], pos[i] > since) >= with;
-      __syncthreads();
-      red[tid] = n;
-      __syncthreads();
-      if (tid == 0) {
-        for (int i = 1; i < 256; ++i) n += red[i];
-        pick = n >= keep ? with : t;
-      }
-      __syncthreads();
-      t = pick;
+  float *mass_out = a.mass_out + row;
+  int *pos_out = a.key_pos_out + row;
+  int *count = (int *)a.ws + blockIdx.x;
+  Pair *list = (Pair *)((int *)a.ws + (long)a.c.batch * a.c.kvh) +
+               (long)blockIdx.x * pairs;
+  if (keep == len) {
+    for (int i = tid; i < room; i += kEvict) {
+      const float m = i < len ? mass[i] : 0.f;
+      const int p = i < len ? pos[i] : -1;
+      mass_out[i] = m;
+      pos_out[i] = p;
     }
+    if (tid == 0) *count = 0;
+    return;
+  }
+
+  // the oldest position that still counts as recent, less one
+  int newest = INT_MIN;
+  for (int i = tid; i < len; i += kEvict) newest = max(newest, pos[i]);
+  for (int o = 32; o; o >>= 1) newest = max(newest, __shfl_xor(newest, o));
+  if (lane == 0) lds_n[0][0][wave] = newest;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kEvictWaves; ++i) newest = max(newest, lds_n[0][0][i]);
+  const long since = (long)newest - a.recent;
+
+  unsigned key[R];
+  auto load = [&](int part) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = part + r * kEvict + tid;
+      key[r] = i < len ? rank_key(mass[i], pos[i] > since) : 0;
+    }
+  };
+  constexpr int kPart = R * kEvict;
+  if (!MANY) load(0);
+
+  // The keep-th largest key, two bits at a time from the top: of the three
+  // next digits the largest that keeps enough.
+  unsigned t = 0;
+  int need = -1;  // how many of those that equal t stay; -1: not known yet
+  for (int bit = 30; bit >= 0; bit -= 2) {
+    int n[3] = {};
+    for (int part = 0; part < (MANY ? len : 1); part += kPart) {
+      if (MANY) load(part);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int d = 0; d < 3; ++d)
+          n[d] += __popcll(__ballot(key[r] >= (t | (unsigned)(d + 1) << bit)));
+    }
+    const int side = bit >> 1 & 1;
+    if (lane < 3)
+      lds_n[side][lane][wave] = lane == 0 ? n[0] : lane == 1 ? n[1] : n[2];
+    __syncthreads();
+    int c = lane < 48 ? lds_n[side][lane / 16][lane % 16] : 0;
+    c = wave_scan(c);
+    const int c0 = __builtin_amdgcn_readlane(c, 15);
+    const int c1 = __builtin_amdgcn_readlane(c, 31) - c0;
+    const int c2 = __builtin_amdgcn_readlane(c, 47) - c0 - c1;
+    const int d = c2 >= keep ? 3 : c1 >= keep ? 2 : c0 >= keep ? 1 : 0;
+    t |= (unsigned)d << bit;
+    if (d && (d == 3 ? c2 : d == 2 ? c1 : c0) == keep) {
+      t -= 1;  // just those above it
+      need = 0;
+      break;
+    }
+  }
+
+  // Ranks in order of the slots, part by part: of the equal ones, of the
+  // free slots below the budget and of the kept rows above it.
+  auto before = [&](int which, int r, int &all) {  // this wave's pass r
+    int sum = 0, own = 0;
+    all = 0;
+    for (int i = lane; i < R * kEvictWaves; i += 64) {
+      const int x = (&lds_c[which][0][0])[i];
+      sum += x;
+      if (i < r * kEvictWaves + wave) own += x;
+    }
+    all = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+    return __builtin_amdgcn_readlane(wave_scan(own), 63);
+  };
+  if (need < 0) {
     int over = 0;
-    for (int i = tid; i < len; i += 256)
-      over += rank_key(mass[i], pos[i] > since) > t;
-    __syncthreads();
-    red[tid] = over;
-    __syncthreads();
-    if (tid == 0) {
-      for (int i = 1; i < 256; ++i) over += red[i];
-      need = keep - over;  // of those that equal t, the first ones stay
-      int ties = 0, holes = 0, movers = 0;
-      for (int i = 0; i < len; ++i) {
-        const unsigned key = rank_key(mass[i], pos[i] > since);
-        const bool stays = key > t || (key == t && ties++ < need);
-        if (!stays && i < keep) list[2 * holes++] = i;
-        if (stays && i >= keep) list[2 * movers++ + 1] = i;
-      }
-      *count = movers;
+    for (int part = 0; part < (MANY ? len : 1); part += kPart) {
+      if (MANY) load(part);
+#pragma unroll
+      for (int r = 0; r < R; ++r) over += __popcll(__ballot(key[r] > t));
     }
-  } else if (tid == 0) {
-    *count = 0;
+    __syncthreads();
+    if (lane == 0) lds_n[0][3][wave] = over;
+    __syncthreads();
+    over = 0;
+#pragma unroll
+    for (int i = 0; i < kEvictWaves; ++i) over += lds_n[0][3][i];
+    need = keep - over;
+  }
+  int ties = 0, holes = 0, movers = 0;
+  const unsigned long long below = (1ull << lane) - 1;
+  for (int part = 0; part < (MANY ? len : 1); part += kPart) {
+    if (MANY) load(part);
+    unsigned stays = 0;  // bit r
+    if (need) {
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int n = __popcll(__ballot(key[r] == t));
+        if (lane == 0) lds_c[0][r][wave] = n;
+      }
+      __syncthreads();
+    }
+    int all = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      bool stay = key[r] > t;
+      if (need && __any(key[r] == t)) {
+        const int rank = ties + before(0, r, all) +
+                         __popcll(__ballot(key[r] == t) & below);
+        stay = stay || (key[r] == t && rank < need);
+      }
+      stays |= (unsigned)stay << r;
+    }
+    if (need) {
+      before(0, 0, all);
+      ties += all;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = part + r * kEvict + tid;
+      const bool stay = stays >> r & 1;
+      const int nh = __popcll(__ballot(i < keep && !stay));
+      const int nm = __popcll(__ballot(i >= keep && stay));
+      if (lane == 0) lds_c[1][r][wave] = nh, lds_c[2][r][wave] = nm;
+    }
+    __syncthreads();
+    int all_h, all_m;
+    before(1, 0, all_h);
+    before(2, 0, all_m);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = part + r * kEvict + tid;
+      const bool stay = stays >> r & 1;
+      const bool hole = i < keep && !stay, mover = i >= keep && stay;
+      if (__any(hole)) {
+        const int at = holes + before(1, r, all) +
+                       __popcll(__ballot(hole) & below);
+        if (hole) list[at].to = i;
+      }
+      if (__any(mover)) {
+        const int at = movers + before(2, r, all) +
+                       __popcll(__ballot(mover) & below);
+        if (mover) list[at].from = i;
+      }
+    }
+    holes += all_h;
+    movers += all_m;
+  }
+  if (tid == 0) *count = movers;
+  // Bookkeeping. The list is whole, and all of the old is still there.
+  __threadfence_block();
+  __syncthreads();
+  if (mass_out != mass)
+    for (int i = tid; i < keep; i += kEvict) mass_out[i] = mass[i];
+  if (pos_out != pos)
+    for (int i = tid; i < keep; i += kEvict) pos_out[i] = pos[i];
+  __syncthreads();
+  for (int i = tid; i < movers; i += kEvict) {
+    const Pair p = list[i];
+    mass_out[p.to] = mass[p.from];
+    pos_out[p.to] = pos[p.from];
+  }
+  __syncthreads();
+  for (int i = keep + tid; i < room; i += kEvict) {
+    mass_out[i] = 0.f;
+    pos_out[i] = -1;
   }
 }
 
+// Sixteen bytes of a key's and of a value's row per thread. Lengths are
+// written here, since the launch before reads the old ones, which may be the
+// same array.
 __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a, int pairs) {
-  const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const int room = a.c.room(), len = a.c.len(b);
-  const int keep = min(len, a.budget);
-  const long row = ((long)b * a.c.kvh + h) * room;
-  const int n = ((const int *)a.ws)[(long)b * a.c.kvh + h];
-  const int *list = (const int *)a.ws + (long)a.c.batch * a.c.kvh +
-                    ((long)b * a.c.kvh + h) * pairs * 2;
-  if (a.mass_out != a.mass)
-    for (int i = tid; i < keep; i += 256) a.mass_out[row + i] = a.mass[row + i];
-  if (a.key_pos_out != a.key_pos)
-    for (int i = tid; i < keep; i += 256)
-      a.key_pos_out[row + i] = a.key_pos[row + i];
-  __syncthreads();
-  for (int i = tid; i < n; i += 256) {
-    const int to = list[2 * i], from = list[2 * i + 1];
-    a.mass_out[row + to] = a.mass[row + from];
-    a.key_pos_out[row + to] = a.key_pos[row + from];
-  }
-  __syncthreads();
-  for (int i = keep + tid; i < room; i += 256) {
-    a.mass_out[row + i] = 0.f;
-    a.key_pos_out[row + i] = -1;
-  }
+  const int b = blockIdx.x / a.c.kvh, h = blockIdx.x % a.c.kvh;
+  const int tid = threadIdx.x;
+  const int n = min(((const int *)a.ws)[blockIdx.x] - (int)blockIdx.y * kPairs,
+                    kPairs);
+  const Pair *list = (const Pair *)((const int *)a.ws +
+                                    (long)a.c.batch * a.c.kvh) +
+                     (long)blockIdx.x * pairs + (long)blockIdx.y * kPairs;
   const int chunks = a.c.d / 8;
+#pragma unroll 4
   for (int i = tid; i < n * chunks; i += 256) {
-    const int to = list[i / chunks * 2], from = list[i / chunks * 2 + 1];
-    const long pt = a.c.page(b, to), pf = a.c.page(b, from);
+    const Pair p = list[i / chunks];
+    const long pt = a.c.page(b, p.to), pf = a.c.page(b, p.from);
     if (pt < 0 || pf < 0) continue;
-    const int c = i % chunks * 8, rt = to % a.c.block, rf = from % a.c.block;
+    const int c = i % chunks * 8;
+    const int rt = (unsigned)p.to % (unsigned)a.c.block;
+    const int rf = (unsigned)p.from % (unsigned)a.c.block;
     bf16 *k = (bf16 *)a.c.k + h * a.c.k_head + c;
     bf16 *v = (bf16 *)a.c.v + h * a.c.v_head + c;
-    *(u32x4 *)(k + pt * a.c.k_page + rt * a.c.k_row) =
-        *(u32x4 *)(k + pf * a.c.k_page + rf * a.c.k_row);
-    *(u32x4 *)(v + pt * a.c.v_page + rt * a.c.v_row) =
-        *(u32x4 *)(v + pf * a.c.v_page + rf * a.c.v_row);
+    const u32x4 kr = *(const u32x4 *)(k + pf * a.c.k_page + rf * a.c.k_row);
+    const u32x4 vr = *(const u32x4 *)(v + pf * a.c.v_page + rf * a.c.v_row);
+    *(u32x4 *)(k + pt * a.c.k_page + rt * a.c.k_row) = kr;
+    *(u32x4 *)(v + pt * a.c.v_page + rt * a.c.v_row) = vr;
   }
-}
-
-// Lengths last: the kernels before it read the old ones, which may be the
-// same array.
-__global__ __launch_bounds__(256) void k_evict_lens(EvictArgs a) {
-  const int b = blockIdx.x * 256 + threadIdx.x;
-  if (b >= a.c.batch) return;
-  const int keep = min(a.c.len(b), a.budget);
-  if (a.c.lens.is64) ((long *)a.lens_out)[b] = keep;
-  else ((int *)a.lens_out)[b] = keep;
+  if (h == 0 && blockIdx.y == 0 && tid == 0) {
+    const int keep = min(a.c.len(b), a.budget);
+    if (a.c.lens.is64) ((long *)a.lens_out)[b] = keep;
+    else ((int *)a.lens_out)[b] = keep;
+  }
 }
 
 }  // namespace
@@ -802,22 +929,34 @@ void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
                 : decode<bf16, 128>(a, w, stream);
 }
 
-size_t kv_evict_workspace(int batch, int kvh, long room, int budget) {
+static int evict_pairs(long room, int budget) {  // most rows that can move
   const long pairs = budget < room - budget ? budget : room - budget;
-  return (size_t)batch * kvh * (1 + 2 * (pairs > 0 ? pairs : 0)) *
-         sizeof(int);
+  return (int)(pairs > 0 ? pairs : 0);
+}
+
+size_t kv_evict_workspace(int batch, int kvh, long room, int budget) {
+  return (size_t)batch * kvh *
+         (sizeof(int) + evict_pairs(room, budget) * sizeof(Pair));
 }
 
 void launch_kv_evict(const EvictArgs &a, hipStream_t stream) {
   if (!a.c.batch) return;
-  const int room = a.c.max_blocks * a.c.block;
-  const int pairs = max(0, min(a.budget, room - a.budget));
-  const dim3 grid(a.c.batch, a.c.kvh);
-  k_evict_select<<<grid, 256, 0, stream>>>(a, pairs);
+  const int room = a.c.room(), pairs = evict_pairs(room, a.budget);
+  const long rows = (long)a.c.batch * a.c.kvh;
+  const long parts = (pairs + kPairs - 1) / kPairs;
+  if (rows > 0x7fffffffL || parts > 65535 || room > 1 << 30)
+    throw std::runtime_error("kv_evict: too many sequences, heads or slots");
+  // registers for as many keys as a sequence can have, in steps that each
+  // cost the shorter ones something
+  if (room <= 4 * kEvict)
+    k_evict_select<4, false><<<rows, kEvict, 0, stream>>>(a, pairs);
+  else if (room <= 16 * kEvict)
+    k_evict_select<16, false><<<rows, kEvict, 0, stream>>>(a, pairs);
+  else
+    k_evict_select<16, true><<<rows, kEvict, 0, stream>>>(a, pairs);
   launched("kv_evict");
+  const dim3 grid((unsigned)rows, (unsigned)(parts ? parts : 1));
   k_evict_move<<<grid, 256, 0, stream>>>(a, pairs);
-  launched("kv_evict");
-  k_evict_lens<<<(a.c.batch + 255) / 256, 256, 0, stream>>>(a);
   launched("kv_evict");
 }
 
