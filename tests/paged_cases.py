@@ -210,6 +210,12 @@ EVICT = {
                     missing=[(0, 1), (0, 5)]),
     "long": dict(lens=[5000, 1300], kvh=1, budget=1200, recent=100, d=8,
                  block=128),
+    "part_equal": dict(lens=[4097, 16384], kvh=1, budget=4000, recent=50, d=8,
+                       block=128, ties=True),
+    "very_long": dict(lens=[40000, 16500, 9], kvh=1, budget=16400, recent=300,
+                      d=8, block=128),
+    "very_long_ties": dict(lens=[36000], kvh=1, budget=17000, recent=0, d=8,
+                           block=128, ties=True),
     "roomy": dict(lens=[30, 20], kvh=2, budget=1 << 30, recent=7),
     "past_room": dict(lens=[48], kvh=1, budget=20, recent=3, tell=[1 << 50],
                       spare=0),

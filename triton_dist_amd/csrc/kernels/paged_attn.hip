@@ -608,8 +608,8 @@ __global__ __launch_bounds__(256) void k_decode_finish(PagedDecodeArgs a,
 //
 // Two launches: a workgroup per sequence and key head finds what stays, does
 // the bookkeeping and lists which row goes where; then all the card moves
-// rows. Bound by latency in the first (a dozen passes over registers with a
-// barrier each), by the rows' bytes in the second. Rows that stay below the
+// rows. Bound by latency in the first (up to four counts of the keys in
+// LDS, each with its barriers), by the rows' bytes in the second. Rows that stay below the
 // budget are not touched, so the steady state, one row over, moves one.
 // ---------------------------------------------------------------------------
 // Order of what stays: slots of the `recent` newest positions first, then
@@ -636,7 +636,7 @@ struct Pair {
 template <int R, bool MANY>
 __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
                                                          int pairs) {
-  __shared__ int lds_n[2][4][kEvictWaves];
+  __shared__ int lds_n[kEvictWaves], hist[256];
   __shared__ int lds_c[3][R][kEvictWaves];
   const int b = blockIdx.x / a.c.kvh, h = blockIdx.x % a.c.kvh;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -661,54 +661,84 @@ __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
     return;
   }
 
-  // the oldest position that still counts as recent, less one
-  int newest = INT_MIN;
-  for (int i = tid; i < len; i += kEvict) newest = max(newest, pos[i]);
-  for (int o = 32; o; o >>= 1) newest = max(newest, __shfl_xor(newest, o));
-  if (lane == 0) lds_n[0][0][wave] = newest;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kEvictWaves; ++i) newest = max(newest, lds_n[0][0][i]);
-  const long since = (long)newest - a.recent;
-
+  // positions from the first one on count as recent
   unsigned key[R];
+  long since = 0;
+  constexpr int kPart = R * kEvict;
+  {
+    int newest = INT_MIN, p[R];
+    float m[R];
+    for (int part = 0; part < (MANY ? len : 1); part += kPart)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int i = part + r * kEvict + tid;
+        p[r] = i < len ? pos[i] : INT_MIN;
+        if (!MANY) m[r] = i < len ? mass[i] : 0.f;
+        newest = max(newest, p[r]);
+      }
+    for (int o = 32; o; o >>= 1) newest = max(newest, __shfl_xor(newest, o));
+    if (lane == 0) lds_n[wave] = newest;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEvictWaves; ++i) newest = max(newest, lds_n[i]);
+    since = (long)newest - a.recent + 1;
+    if (!MANY)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        key[r] = r * kEvict + tid < len ? rank_key(m[r], p[r] >= since) : 0;
+  }
   auto load = [&](int part) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int i = part + r * kEvict + tid;
-      key[r] = i < len ? rank_key(mass[i], pos[i] > since) : 0;
+      key[r] = i < len ? rank_key(mass[i], pos[i] >= since) : 0;
     }
   };
-  constexpr int kPart = R * kEvict;
-  if (!MANY) load(0);
 
-  // The keep-th largest key, two bits at a time from the top: of the three
-  // next digits the largest that keeps enough.
+  // The keep-th largest key, eight bits at a time from the top, by counts of
+  // the keys that agree so far. Of those that equal it, `need` stay.
   unsigned t = 0;
-  int need = -1;  // how many of those that equal t stay; -1: not known yet
-  for (int bit = 30; bit >= 0; bit -= 2) {
-    int n[3] = {};
+  int need = keep;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    __syncthreads();
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
     for (int part = 0; part < (MANY ? len : 1); part += kPart) {
       if (MANY) load(part);
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int d = 0; d < 3; ++d)
-          n[d] += __popcll(__ballot(key[r] >= (t | (unsigned)(d + 1) << bit)));
+      for (int r = 0; r < R; ++r) {
+        const bool in = key[r] && (shift == 24 || (key[r] ^ t) >> shift < 256);
+        const int bin = key[r] >> shift & 255;
+        const unsigned long long who = __ballot(in);
+        if (!who) continue;
+        // often all lanes want one bin: weights of one size, recent slots
+        const int first = __builtin_amdgcn_readlane(bin, __builtin_ctzll(who));
+        if (__ballot(in && bin == first) == who) {
+          if (lane == 0) atomicAdd(&hist[first], (int)__popcll(who));
+        } else if (in) {
+          atomicAdd(&hist[bin], 1);
+        }
+      }
     }
-    const int side = bit >> 1 & 1;
-    if (lane < 3)
-      lds_n[side][lane][wave] = lane == 0 ? n[0] : lane == 1 ? n[1] : n[2];
     __syncthreads();
-    int c = lane < 48 ? lds_n[side][lane / 16][lane % 16] : 0;
-    c = wave_scan(c);
-    const int c0 = __builtin_amdgcn_readlane(c, 15);
-    const int c1 = __builtin_amdgcn_readlane(c, 31) - c0;
-    const int c2 = __builtin_amdgcn_readlane(c, 47) - c0 - c1;
-    const int d = c2 >= keep ? 3 : c1 >= keep ? 2 : c0 >= keep ? 1 : 0;
-    t |= (unsigned)d << bit;
-    if (d && (d == 3 ? c2 : d == 2 ? c1 : c0) == keep) {
-      t -= 1;  // just those above it
+    // lane i has bins 255 - 4 i down, so sums come from the largest
+    int n[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += n[i] = hist[255 - 4 * lane - i];
+    int above = wave_scan(sum) - sum;
+    const int at = __builtin_ctzll(__ballot(above + sum >= need));
+    above = __builtin_amdgcn_readlane(above, at);
+    int digit = 255 - 4 * at, in_bin = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int x = __builtin_amdgcn_readlane(n[i], at);
+      if (in_bin == 0 && above + x >= need) in_bin = x, digit -= i;
+      else if (in_bin == 0) above += x;
+    }
+    need -= above;
+    t |= (unsigned)digit << shift;
+    if (in_bin == need) {
+      t -= 1;  // those above it are just enough
       need = 0;
       break;
     }
@@ -727,21 +757,6 @@ __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
     all = __builtin_amdgcn_readlane(wave_scan(sum), 63);
     return __builtin_amdgcn_readlane(wave_scan(own), 63);
   };
-  if (need < 0) {
-    int over = 0;
-    for (int part = 0; part < (MANY ? len : 1); part += kPart) {
-      if (MANY) load(part);
-#pragma unroll
-      for (int r = 0; r < R; ++r) over += __popcll(__ballot(key[r] > t));
-    }
-    __syncthreads();
-    if (lane == 0) lds_n[0][3][wave] = over;
-    __syncthreads();
-    over = 0;
-#pragma unroll
-    for (int i = 0; i < kEvictWaves; ++i) over += lds_n[0][3][i];
-    need = keep - over;
-  }
   int ties = 0, holes = 0, movers = 0;
   const unsigned long long below = (1ull << lane) - 1;
   for (int part = 0; part < (MANY ? len : 1); part += kPart) {
