@@ -85,6 +85,13 @@ DECODE = {
     "negative": dict(lens=[90, 3], qh=4, kvh=2, d=64, block=16, scale=-0.4),
     "batch": dict(lens=[(i * 37) % 90 for i in range(70)], qh=4, kvh=2,
                   d=64, block=16),
+    "big_batch": dict(lens=[(i * 37) % 70 for i in range(515)], qh=3, kvh=3,
+                      d=64, block=16, slopes=True),
+    "big_ragged": dict(lens=[1900] + [(i * 7) % 5 for i in range(300)]
+                       + [700] + [0] * 230, qh=10, kvh=1, d=128, block=64,
+                       mass=True),
+    "big_heads": dict(lens=[(i * 11) % 40 for i in range(130)], qh=34,
+                      kvh=17, d=64, block=8),
 }
 
 

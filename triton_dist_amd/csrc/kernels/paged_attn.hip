@@ -120,6 +120,7 @@ constexpr int kSlots = 512;            // workgroups that the card holds
 constexpr int kFew = 6;                // steps that a workgroup starts for
 
 template <typename T> using vec8 = __attribute__((ext_vector_type(8))) T;
+template <typename T> using vec4 = __attribute__((ext_vector_type(4))) T;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 // at any float's address
@@ -234,10 +235,12 @@ struct DecodeWork {
   float *sum;     // [chunks, qh]: log2 of a chunk's sum
   int *plan;      // [batch, 2]: a sequence's chunks, its first further one
   float *logits;  // [batch, qh, room], in units of log2, where weights are
-  int target, least, groups;
+  int target, least, groups, waves;
 };
 
-template <typename T, int D>
+// W waves of a workgroup share a key head's chunk: all four, joined at the
+// end, or each has a key head of its own.
+template <typename T, int D, int W>
 __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
                                                          DecodeWork w) {
   constexpr int kC = D / 32, kT = D / 16;  // pieces of a row, tiles of it
@@ -251,8 +254,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int n = lane & 15, qd = lane >> 4;
+  constexpr int kStride = W * kTile;
   const int per = a.c.kvh * w.groups;
-  const int id = blockIdx.x / per;
+  const int blocks = W == 4 ? per : (per + 3) / 4;  // of a chunk
+  const int id = blockIdx.x / blocks;
   Chunk ch{id, 0, 0, 1, w.least};
   if (id >= a.c.batch) {
     if (!find_further(a.c, find_cut(a.c, w.target, w.least, found),
@@ -265,12 +270,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
       ch.count = chunks_of(ch.len, ch.steps);
     }
   }
-  if (tid == 0 && blockIdx.x % per == 0) {
+  if (tid == 0 && blockIdx.x % blocks == 0) {
     if (ch.first == 0) w.plan[2 * ch.b] = ch.count;
     if (ch.first == 1) w.plan[2 * ch.b + 1] = id;
   }
-  const int kh = blockIdx.x % per / w.groups;
-  const int group = blockIdx.x % per % w.groups;
+  const int share = W == 4 ? blockIdx.x % per : blockIdx.x % blocks * 4 + wave;
+  if (W == 1 && share >= per) return;  // no barrier follows
+  const int kh = share / w.groups, group = share % w.groups;
   const int g = a.qh / a.c.kvh;
   const int h0 = kh * g + group * 16;       // first query head here
   const int heads = min(16, g - group * 16);
@@ -348,15 +354,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
   float m = -INFINITY, l = 0.f;  // m of all quads alike, l of this lane
   f32x4 acc[kT] = {};
   T *vl = (T *)lds[wave];
-  int base = k0 + wave * kTile;
+  int base = k0 + (W == 4 ? wave * kTile : 0);
   if (base < k1) {
     look_up(base);
     load_k(base);
     load_v(base);
-    look_up(base + kStep);
+    look_up(base + kStride);
   }
-  for (; base < k1; base += kStep) {
-    const bool more = base + kStep < k1;
+  for (; base < k1; base += kStride) {
+    const bool more = base + kStride < k1;
     f32x4 s[2] = {};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -389,9 +395,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
         *(vec8<T> *)(vl + (16 * t + n) * kRow + c * 32 + qd * 8) = vf[t][c];
     wave_fence();
     if (more) {
-      load_k(base + kStep);
-      load_v(base + kStep);
-      look_up(base + 2 * kStep);
+      load_k(base + kStride);
+      load_v(base + kStride);
+      look_up(base + 2 * kStride);
     }
     // scores, in units of log2
     if (a.s.softcap > 0.f) {
@@ -472,9 +478,32 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
     wave_fence();  // the next tile's values go where these were
   }
 
-  // join the four waves
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
+  if (W == 1) {
+    if (n >= heads) return;
+    const float r = l == 0.f ? 0.f : 1.f / l;
+    const float lse = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+    const long at = (long)id * a.qh + h0 + n, to = (long)b * a.qh + h0 + n;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      acc[t] *= r;
+      if (ch.count == 1) {
+        vec4<T> o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = (T)acc[t][i];
+        *(vec4<T> *)((T *)a.out + to * D + t * 16 + qd * 4) = o;
+      } else {
+        *(f32x4 *)(w.part + at * D + t * 16 + qd * 4) = acc[t];
+      }
+    }
+    if (qd == 0) {
+      w.sum[at] = lse;
+      if (ch.count == 1 && a.lse) a.lse[to] = lse * kLn2;
+    }
+    return;
+  }
+  // join the four waves
   float *ol = (float *)lds[wave];
 #pragma unroll
   for (int t = 0; t < kT; ++t)
@@ -894,8 +923,14 @@ void launch_paged_append(const PagedArgs &a, const void *k, long k_tok,
 static DecodeWork decode_work(int batch, int qh, int kvh) {
   DecodeWork w{};
   w.groups = (qh / kvh + 15) / 16;
-  const int per = kvh * w.groups;
-  w.target = (kSlots + per - 1) / per;
+  const int per = kvh * w.groups, own = (per + 3) / 4;
+  // A wave to a key head where the sequences fill the card that way: it
+  // needs no joining (512 sequences of 131 keys and 8 heads: 65 us for 83).
+  w.waves = (long)batch * own >= kSlots ? 1 : 4;
+  const int blocks = w.waves == 1 ? own : per;
+  w.target = (kSlots + blocks - 1) / blocks;
+  // Under two steps a chunk's start costs more than its keys: one sequence of
+  // 700 keys took 15 us in chunks of two and the join, 20 us in one piece.
   w.least = 2;
   return w;
 }
@@ -911,10 +946,14 @@ size_t paged_decode_workspace(int batch, int qh, int kvh, int d, long room,
 template <typename T, int D>
 static void decode(const PagedDecodeArgs &a, const DecodeWork &w,
                    hipStream_t stream) {
-  const long blocks = (2 * (long)w.target + a.c.batch) * a.c.kvh * w.groups;
+  const int per = a.c.kvh * w.groups;
+  const long blocks = (2 * (long)w.target + a.c.batch) *
+                      (w.waves == 1 ? (per + 3) / 4 : per);
   if (blocks > 0x7fffffffL)
     throw std::runtime_error("paged_decode: too many sequences and heads");
-  k_paged_decode<T, D><<<dim3((unsigned)blocks), 256, 0, stream>>>(a, w);
+  const dim3 grid((unsigned)blocks);
+  if (w.waves == 1) k_paged_decode<T, D, 1><<<grid, 256, 0, stream>>>(a, w);
+  else k_paged_decode<T, D, 4><<<grid, 256, 0, stream>>>(a, w);
   launched("paged_decode");
   // nothing to join where no sequence can have two chunks
   const int spans = a.mass ? (a.c.room() + kSpan - 1) / kSpan : 0;
