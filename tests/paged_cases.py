@@ -90,6 +90,15 @@ DECODE = {
     "big_ragged": dict(lens=[1900] + [(i * 7) % 5 for i in range(300)]
                        + [700] + [0] * 230, qh=10, kvh=1, d=128, block=64,
                        mass=True),
+    "bigger_batch": dict(lens=[(i * 37) % 33 for i in range(1024)] + [700],
+                         qh=6, kvh=3, d=64, block=16, mass=True),
+    "bigger_ragged": dict(lens=[(i * 97) % 601 for i in range(24)], qh=64,
+                          kvh=64, d=64, block=32, slopes=True),
+    "bigger_mass": dict(lens=[900, 0, 385, 1, 640, 513, 129, 770], qh=100,
+                        kvh=100, d=128, block=64, mass=True, moved=True,
+                        slopes=True),
+    "bigger_groups": dict(lens=[3000, 2500], qh=2 * 34, kvh=34, d=64,
+                          block=64, softcap=9.0),
     "big_heads": dict(lens=[(i * 11) % 40 for i in range(130)], qh=34,
                       kvh=17, d=64, block=8),
 }

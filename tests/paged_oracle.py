@@ -48,16 +48,11 @@ def attend(q, k, v, scale, softcap, bias, dtype):
 def gather(pool, table_row, slots, head):
     """Rows of one sequence's slots and whether their pages are there."""
     block = pool.shape[1]
-    rows, there = [], []
-    for s in slots:
-        page = int(table_row[s // block])
-        ok = 0 <= page < pool.shape[0]
-        there.append(ok)
-        if ok:
-            rows.append(pool[page, s % block, head])
-    rows = torch.stack(rows).double() if rows else torch.zeros(
-        0, pool.shape[3], dtype=torch.float64)
-    return rows, there
+    slots = torch.tensor(list(slots), dtype=torch.long)
+    page = table_row.long()[slots // block]
+    there = (page >= 0) & (page < pool.shape[0])
+    rows = pool[page[there], slots[there] % block, head].double()
+    return rows, there.tolist()
 
 
 def decode(q, k_pool, v_pool, table, lens, scale=None, softcap=0.0,

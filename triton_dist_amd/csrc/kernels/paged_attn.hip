@@ -96,11 +96,11 @@ __global__ __launch_bounds__(256) void k_paged_append(
 //
 // Bound by reading K and V once. The batch's keys are cut into chunks of
 // equal length on the device, from the lengths as they are, so a long
-// sequence among short ones is spread over the card as well; a workgroup
-// takes one chunk of one key head and up to 16 of its query heads.
+// sequence among short ones is spread over the card as well. A wave takes a
+// key head of one and up to 16 of its query heads, or a quarter of the tiles
+// of that (find_cut).
 //
-// In a workgroup each of the four waves goes through 32-key tiles of its
-// own, without a barrier. S^T = K Q^T and O^T = V^T P^T, so that a lane
+// A wave goes through its 32-key tiles without a barrier. S^T = K Q^T and O^T = V^T P^T, so that a lane
 // holds the scores of one query head all the way: lane (n, qd) = (lane & 15,
 // lane >> 4) gets from the 16x16x32 matrix instructions the scores of head n
 // and keys 16 t + 4 qd + i, which are the elements that the second product
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void k_paged_append(
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 32;              // keys of a wave's step
-constexpr int kStep = 4 * kTile;       // keys of a workgroup's step
+constexpr int kStep = 4 * kTile;       // keys that chunks are measured in
 constexpr int kSlots = 512;            // workgroups that the card holds
 constexpr int kFew = 6;                // steps that a workgroup starts for
 
@@ -149,70 +149,76 @@ TD_DEV void wave_fence() {
 struct Chunk {
   int b, len;        // sequence and its length
   int first, count;  // this chunk's number among the sequence's, how many
-  int steps;         // of kStep keys, a chunk's length
 };
 
-// A sequence's first chunk has the sequence's number, so that finding it
-// takes nothing; the further ones are numbered behind those, sequence by
-// sequence, and are found by a sum over the batch. All of a workgroup of 256
-// threads calls these.
-struct Cut {
-  int steps;  // a chunk's length
-  int each;   // sequences that a thread sums over
+// Where a call keeps what its kernels hand on.
+struct DecodeWork {
+  float *part;    // [chunks, qh, d]: outputs of one chunk among several
+  float *sum;     // [chunks, qh]: log2 of a chunk's sum
+  int *plan;      // [batch, 2]: a sequence's chunks, its first further one
+  float *logits;  // [batch, qh, room], in units of log2, where weights are
+  int groups;     // of up to 16 query heads of a key head
+  int apart;      // waves never share a chunk
+  int least;      // steps of a chunk
+  int joins;      // workgroups that join a key head's query heads
 };
-// How long chunks are, from the lengths of the whole batch.
-TD_DEV Cut find_cut(const PagedArgs &c, int target, int least, int *lds) {
-  const int tid = threadIdx.x;
-  Cut cut;
-  cut.each = (c.batch + 255) / 256;
+
+// How the batch's keys are cut, from the lengths as they are. A sequence's
+// first chunk has the sequence's number; further ones are numbered behind
+// those, sequence by sequence. All of a workgroup of 256 threads calls this.
+struct Cut {
+  int steps;   // a chunk's length
+  int most;    // further chunks at most
+  bool shared; // a workgroup's waves share one head's chunk
+};
+TD_DEV int steps_of(int len) { return (len + kStep - 1) / kStep; }
+TD_DEV int chunks_of(int len, int steps) {
+  return max(1, (steps_of(len) + steps - 1) / steps);
+}
+TD_DEV Cut find_cut(const PagedArgs &c, const DecodeWork &w, int *lds) {
+  const int tid = threadIdx.x, each = (c.batch + 255) / 256;
   int sum = 0;
-  for (int i = tid * cut.each; i < min((tid + 1) * cut.each, c.batch); ++i)
-    sum += (c.len(i) + kStep - 1) / kStep;
+  for (int i = tid * each; i < min((tid + 1) * each, c.batch); ++i)
+    sum += steps_of(c.len(i));
   sum = wave_scan(sum);
-  __syncthreads();
   if ((tid & 63) == 63) lds[tid >> 6] = sum;
   __syncthreads();
   const long total = (long)lds[0] + lds[1] + lds[2] + lds[3];
-  // One chunk a workgroup that the card holds, where that makes short ones
-  // (starting takes as long as a few steps); else two, which even out what
+  const int per = c.kvh * w.groups, own = (per + 3) / 4;
+  Cut cut;
+  // Few steps for a workgroup: its waves share one, which is done soonest
+  // (32 sequences of up to 4100 keys, 4 key heads: 24 us for 28). Else each
+  // wave has a key head of its own, so that a workgroup reads neighbouring
+  // heads' rows and joins nothing (48 of up to 16384, 8 key heads: 203 us
+  // for 228), in twice the chunks that the card holds, which evens out what
   // ragged sequences leave over.
-  cut.steps = (int)((total + target - 1) / target);
-  if (cut.steps > kFew) cut.steps = (int)((total + 2 * target - 1) /
-                                          (2 * target));
-  cut.steps = max(least, cut.steps);
+  cut.shared = !w.apart && total * per < kFew * kSlots;
+  const long target = cut.shared ? (kSlots + per - 1) / per
+                                 : (2 * kSlots + own - 1) / own;
+  cut.steps = max(w.least, (int)((total + target - 1) / target));
+  cut.most = (int)(total / cut.steps);
   return cut;
 }
-TD_DEV int chunks_of(int len, int steps) {
-  return max(1, ((len + kStep - 1) / kStep + steps - 1) / steps);
-}
-// The further chunks before this thread's sequences; `all` of the batch.
-TD_DEV int further_before(const PagedArgs &c, const Cut &cut, int *lds,
-                          int &all) {
-  const int tid = threadIdx.x;
+// The further chunk `at`; false where there are not so many.
+TD_DEV bool find_further(const PagedArgs &c, const Cut &cut, int at,
+                         int *lds, Chunk &out) {
+  if (at >= cut.most) return false;
+  const int tid = threadIdx.x, each = (c.batch + 255) / 256;
   int own = 0;
-  for (int i = tid * cut.each; i < min((tid + 1) * cut.each, c.batch); ++i)
+  for (int i = tid * each; i < min((tid + 1) * each, c.batch); ++i)
     own += chunks_of(c.len(i), cut.steps) - 1;
   const int upto = wave_scan(own);
   __syncthreads();
   if ((tid & 63) == 63) lds[tid >> 6] = upto;
   __syncthreads();
-  int before = upto - own;
-  all = 0;
+  int before = upto - own, all = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (i < tid >> 6) before += lds[i];
     all += lds[i];
   }
-  return before;
-}
-// The further chunk `at`; false where there are not so many.
-TD_DEV bool find_further(const PagedArgs &c, const Cut &cut, int at,
-                         int *lds, Chunk &out) {
-  int all;
-  int before = further_before(c, cut, lds, all);
   if (at >= all) return false;
-  const int tid = threadIdx.x;
-  for (int i = tid * cut.each; i < min((tid + 1) * cut.each, c.batch); ++i) {
+  for (int i = tid * each; i < min((tid + 1) * each, c.batch); ++i) {
     const int n = chunks_of(c.len(i), cut.steps) - 1;
     if (at >= before && at < before + n) {
       lds[4] = i;
@@ -224,23 +230,11 @@ TD_DEV bool find_further(const PagedArgs &c, const Cut &cut, int at,
   out.b = lds[4];
   out.first = lds[5];
   out.len = c.len(out.b);
-  out.steps = cut.steps;
   out.count = chunks_of(out.len, cut.steps);
   return true;
 }
 
-// Where a call keeps what its kernels hand on.
-struct DecodeWork {
-  float *part;    // [chunks, qh, d]: outputs of one chunk among several
-  float *sum;     // [chunks, qh]: log2 of a chunk's sum
-  int *plan;      // [batch, 2]: a sequence's chunks, its first further one
-  float *logits;  // [batch, qh, room], in units of log2, where weights are
-  int target, least, groups, waves;
-};
-
-// W waves of a workgroup share a key head's chunk: all four, joined at the
-// end, or each has a key head of its own.
-template <typename T, int D, int W>
+template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
                                                          DecodeWork w) {
   constexpr int kC = D / 32, kT = D / 16;  // pieces of a row, tiles of it
@@ -254,36 +248,33 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int n = lane & 15, qd = lane >> 4;
-  constexpr int kStride = W * kTile;
+  const Cut cut = find_cut(a.c, w, found);
   const int per = a.c.kvh * w.groups;
-  const int blocks = W == 4 ? per : (per + 3) / 4;  // of a chunk
+  const int blocks = cut.shared ? per : (per + 3) / 4;  // of a chunk
   const int id = blockIdx.x / blocks;
-  Chunk ch{id, 0, 0, 1, w.least};
+  Chunk ch{id, 0, 0, 1};
   if (id >= a.c.batch) {
-    if (!find_further(a.c, find_cut(a.c, w.target, w.least, found),
-                      id - a.c.batch, found, ch))
-      return;
+    if (!find_further(a.c, cut, id - a.c.batch, found, ch)) return;
   } else {
     ch.len = a.c.len(id);
-    if (ch.len > w.least * kStep) {
-      ch.steps = find_cut(a.c, w.target, w.least, found).steps;
-      ch.count = chunks_of(ch.len, ch.steps);
-    }
+    ch.count = chunks_of(ch.len, cut.steps);
   }
   if (tid == 0 && blockIdx.x % blocks == 0) {
     if (ch.first == 0) w.plan[2 * ch.b] = ch.count;
     if (ch.first == 1) w.plan[2 * ch.b + 1] = id;
   }
-  const int share = W == 4 ? blockIdx.x % per : blockIdx.x % blocks * 4 + wave;
-  if (W == 1 && share >= per) return;  // no barrier follows
+  const int stride = cut.shared ? kStep : kTile;
+  const int share = cut.shared ? blockIdx.x % per
+                               : blockIdx.x % blocks * 4 + wave;
+  if (share >= per) return;  // and with it no barrier follows
   const int kh = share / w.groups, group = share % w.groups;
   const int g = a.qh / a.c.kvh;
   const int h0 = kh * g + group * 16;       // first query head here
   const int heads = min(16, g - group * 16);
   const int b = ch.b;
-  const long cut = (long)ch.steps * kStep;
-  const int k0 = (int)(ch.first * cut);
-  const int k1 = (int)min((long)ch.len, k0 + cut);
+  const long long_cut = (long)cut.steps * kStep;
+  const int k0 = (int)(ch.first * long_cut);
+  const int k1 = (int)min((long)ch.len, k0 + long_cut);
 
   vec8<T> qf[kC] = {};
   if (n < heads) {
@@ -354,15 +345,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
   float m = -INFINITY, l = 0.f;  // m of all quads alike, l of this lane
   f32x4 acc[kT] = {};
   T *vl = (T *)lds[wave];
-  int base = k0 + (W == 4 ? wave * kTile : 0);
+  int base = k0 + (cut.shared ? wave * kTile : 0);
   if (base < k1) {
     look_up(base);
     load_k(base);
     load_v(base);
-    look_up(base + kStride);
+    look_up(base + stride);
   }
-  for (; base < k1; base += kStride) {
-    const bool more = base + kStride < k1;
+  for (; base < k1; base += stride) {
+    const bool more = base + stride < k1;
     f32x4 s[2] = {};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -395,9 +386,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
         *(vec8<T> *)(vl + (16 * t + n) * kRow + c * 32 + qd * 8) = vf[t][c];
     wave_fence();
     if (more) {
-      load_k(base + kStride);
-      load_v(base + kStride);
-      look_up(base + 2 * kStride);
+      load_k(base + stride);
+      load_v(base + stride);
+      look_up(base + 2 * stride);
     }
     // scores, in units of log2
     if (a.s.softcap > 0.f) {
@@ -480,7 +471,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
 
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
-  if (W == 1) {
+  if (!cut.shared) {
     if (n >= heads) return;
     const float r = l == 0.f ? 0.f : 1.f / l;
     const float lse = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
@@ -529,12 +520,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
     o *= sum == 0.f ? 0.f : 1.f / sum;
     const float lse = sum == 0.f ? -INFINITY
                                  : top + __builtin_amdgcn_logf(sum);
-    const long at = (long)id * a.qh + h0 + h;
+    const long at = (long)id * a.qh + h0 + h, to = (long)b * a.qh + h0 + h;
     if (ch.count == 1) {
-      T *to = (T *)a.out + ((long)b * a.qh + h0 + h) * D + c;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) to[x] = (T)o[x];
-      if (c == 0 && a.lse) a.lse[(long)b * a.qh + h0 + h] = lse * kLn2;
+      for (int x = 0; x < 4; ++x) ((T *)a.out)[to * D + c + x] = (T)o[x];
+      if (c == 0 && a.lse) a.lse[to] = lse * kLn2;
     } else {
       *(f32x4 *)(w.part + at * D + c) = o;
     }
@@ -543,14 +533,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
 }
 
 // Joins a sequence's chunks and hands out its weights: of the workgroups
-// (sequence, key head, z) the first ones join a query head each, and each
-// further one adds the weights of 1024 slots, from the logits that the first
-// kernel kept.
-constexpr int kSpan = 1024;
+// (sequence, key head, z) the first w.joins share out the query heads, and
+// each further one adds the weights of 1024 slots, from the logits that the
+// first kernel kept.
+constexpr int kSpan = 1024;    // slots
+constexpr int kSpanWaves = 8;
 template <typename T, int D>
-__global__ __launch_bounds__(256) void k_decode_finish(PagedDecodeArgs a,
-                                                       DecodeWork w) {
-  __shared__ float lds_lse[4], lds_o[4][D];
+__global__ __launch_bounds__(64 * kSpanWaves) void k_decode_finish(PagedDecodeArgs a,
+                                                         DecodeWork w) {
+  __shared__ float lds_lse[kSpanWaves], lds_o[kSpanWaves][D];
   const int b = blockIdx.x, kh = blockIdx.y, z = blockIdx.z;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int g = a.qh / a.c.kvh, room = a.c.room();
@@ -558,8 +549,8 @@ __global__ __launch_bounds__(256) void k_decode_finish(PagedDecodeArgs a,
   auto row = [&](int i, int h) {  // a chunk's outputs of a query head
     return (long)(i ? more + i - 1 : b) * a.qh + h;
   };
-  auto lse_of = [&](int h, float &top) {  // the whole wave
-    top = -INFINITY;
+  auto lse_of = [&](int h) {  // the whole wave
+    float top = -INFINITY;
     for (int i = lane; i < count; i += 64)
       top = fmaxf(top, w.sum[row(i, h)]);
     top = wave_max(top);
@@ -570,62 +561,79 @@ __global__ __launch_bounds__(256) void k_decode_finish(PagedDecodeArgs a,
     sum = wave_sum(sum);
     return sum == 0.f ? -INFINITY : safe + __builtin_amdgcn_logf(sum);
   };
-  if (z < g) {
+  if (z < w.joins) {
     if (count == 1) return;
-    const int h = kh * g + z;
-    float top;
-    const float lse = lse_of(h, top);
-    const float safe = lse == -INFINITY ? 0.f : lse;
-    float o[D / 64] = {};
+    // heads of this workgroup, waves to a head, heads at once
+    const int heads = (g + w.joins - 1) / w.joins;
+    const int each = max(1, kSpanWaves / heads), at_once = kSpanWaves / each;
+    for (int x = 0; x < heads; x += at_once) {
+      const int y = x + wave / each, h = kh * g + z * heads + y;
+      const bool live = wave < each * at_once && y < heads &&
+                        z * heads + y < g;
+      if (live) {
+        const float lse = lse_of(h);
+        const float safe = lse == -INFINITY ? 0.f : lse;
+        float o[D / 64] = {};
 #pragma unroll 4
-    for (int i = wave; i < count; i += 4) {
-      const long at = row(i, h);
-      const float r = __builtin_amdgcn_exp2f(w.sum[at] - safe);
+        for (int i = wave % each; i < count; i += each) {
+          const long at = row(i, h);
+          const float r = __builtin_amdgcn_exp2f(w.sum[at] - safe);
 #pragma unroll
-      for (int y = 0; y < D / 64; ++y)
-        o[y] += r * w.part[at * D + lane * (D / 64) + y];
+          for (int c = 0; c < D / 64; ++c)
+            o[c] += r * w.part[at * D + lane * (D / 64) + c];
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          lds_o[wave][lane * (D / 64) + c] = o[c];
+        if (wave % each == 0 && lane == 0 && a.lse)
+          a.lse[(long)b * a.qh + h] = lse * kLn2;
+      }
+      __syncthreads();
+      for (int i = tid; i < at_once * D; i += 64 * kSpanWaves) {
+        const int p = i / D, c = i % D;
+        if (x + p >= heads || z * heads + x + p >= g) continue;
+        float sum = 0.f;
+        for (int v = 0; v < each; ++v) sum += lds_o[p * each + v][c];
+        ((T *)a.out)[((long)b * a.qh + kh * g + z * heads + x + p) * D + c] =
+            (T)sum;
+      }
+      __syncthreads();
     }
-#pragma unroll
-    for (int y = 0; y < D / 64; ++y) lds_o[wave][lane * (D / 64) + y] = o[y];
-    __syncthreads();
-    if (tid < D)
-      ((T *)a.out)[((long)b * a.qh + h) * D + tid] =
-          (T)(lds_o[0][tid] + lds_o[1][tid] + lds_o[2][tid] + lds_o[3][tid]);
-    if (tid == 0 && a.lse) a.lse[(long)b * a.qh + h] = lse * kLn2;
     return;
   }
-  const int len = a.c.len(b);
+  constexpr int kOwn = kSpan / 64 / kSpanWaves;
+  const int len = a.c.len(b), from = (z - w.joins) * kSpan + tid;
   const long plane = ((long)b * a.c.kvh + kh) * room;
-  const int from = (z - g) * kSpan + tid;
-  float sum[kSpan / 256] = {};
-  if ((z - g) * kSpan < len)
-    for (int x = 0; x < g; x += 4) {
-      float s[4][kSpan / 256];
+  float sum[kOwn] = {};
+  if ((z - w.joins) * kSpan < len)
+    for (int x = 0; x < g; x += kSpanWaves) {
+      const float *s = w.logits + ((long)b * a.qh + kh * g + x) * room + from;
+      float logit[kSpanWaves][kOwn];
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
+      for (int y = 0; y < kSpanWaves; ++y)
 #pragma unroll
-        for (int i = 0; i < kSpan / 256; ++i)
-          s[y][i] = x + y < g && from + i * 256 < len
-                        ? w.logits[((long)b * a.qh + kh * g + x + y) * room +
-                                   from + i * 256]
-                        : -INFINITY;
+        for (int i = 0; i < kOwn; ++i) {
+          const int slot = from + i * 64 * kSpanWaves;
+          logit[y][i] = x + y < g && slot < len
+                            ? s[(long)y * room + i * 64 * kSpanWaves]
+                            : -INFINITY;
+        }
+      const float lse = x + wave < g ? lse_of(kh * g + x + wave) : -INFINITY;
       __syncthreads();
-      float top, lse = -INFINITY;
-      if (x + wave < g) lse = lse_of(kh * g + x + wave, top);
       if (lane == 0) lds_lse[wave] = lse;
       __syncthreads();
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
+      for (int y = 0; y < kSpanWaves; ++y) {
         const float total = lds_lse[y];
         if (total == -INFINITY) continue;  // also a head that is not there
 #pragma unroll
-        for (int i = 0; i < kSpan / 256; ++i)
-          sum[i] += __builtin_amdgcn_exp2f(s[y][i] - total);
+        for (int i = 0; i < kOwn; ++i)
+          sum[i] += __builtin_amdgcn_exp2f(logit[y][i] - total);
       }
     }
 #pragma unroll
-  for (int i = 0; i < kSpan / 256; ++i) {
-    const int slot = from + i * 256;
+  for (int i = 0; i < kOwn; ++i) {
+    const int slot = from + i * 64 * kSpanWaves;
     if (slot < room)
       a.mass_out[plane + slot] = slot < len ? a.mass[plane + slot] + sum[i]
                                             : 0.f;
@@ -918,60 +926,62 @@ void launch_paged_append(const PagedArgs &a, const void *k, long k_tok,
   launched("paged_append");
 }
 
-// Chunks are made so that the card is full: kSlots workgroups, of which
-// each sequence may add one that is not.
 static DecodeWork decode_work(int batch, int qh, int kvh) {
   DecodeWork w{};
   w.groups = (qh / kvh + 15) / 16;
-  const int per = kvh * w.groups, own = (per + 3) / 4;
-  // A wave to a key head where the sequences fill the card that way: it
-  // needs no joining (512 sequences of 131 keys and 8 heads: 65 us for 83).
-  w.waves = (long)batch * own >= kSlots ? 1 : 4;
-  const int blocks = w.waves == 1 ? own : per;
-  w.target = (kSlots + blocks - 1) / blocks;
-  // Under two steps a chunk's start costs more than its keys: one sequence of
-  // 700 keys took 15 us in chunks of two and the join, 20 us in one piece.
-  w.least = 2;
+  // so many sequences that there are steps enough, if none is empty
+  w.apart = (long)batch * kvh * w.groups >= kFew * kSlots;
+  w.least = w.apart ? 2 : 1;
+  // a workgroup to a query head, unless so many would take longer to start
+  // than to join (512 sequences, 8 key heads, nothing to join: 17 us)
+  const long most = 4 * kSlots / ((long)batch * kvh);
+  w.joins = (int)max(1L, min((long)(qh / kvh), most));
   return w;
+}
+
+// Chunks at most: those of a cut that is shared and of one that is not, over
+// the blocks that each takes.
+static long decode_chunks(int batch, int kvh, const DecodeWork &w) {
+  const int per = kvh * w.groups, own = (per + 3) / 4;
+  return batch + max((kSlots + per - 1) / per, (2 * kSlots + own - 1) / own);
 }
 
 size_t paged_decode_workspace(int batch, int qh, int kvh, int d, long room,
                               bool mass) {
-  const DecodeWork w = decode_work(batch, qh, kvh);
-  const size_t chunks = 2 * (size_t)w.target + batch;
-  return (chunks * qh * (d + 1) + 2 * (size_t)batch + (mass ? (size_t)batch * qh * room : 0)) *
+  const size_t chunks = decode_chunks(batch, kvh, decode_work(batch, qh, kvh));
+  return (chunks * qh * (d + 1) + 2 * (size_t)batch +
+          (mass ? (size_t)batch * qh * room : 0)) *
          sizeof(float);
 }
 
 template <typename T, int D>
 static void decode(const PagedDecodeArgs &a, const DecodeWork &w,
                    hipStream_t stream) {
-  const int per = a.c.kvh * w.groups;
-  const long blocks = (2 * (long)w.target + a.c.batch) *
-                      (w.waves == 1 ? (per + 3) / 4 : per);
+  const int per = a.c.kvh * w.groups, own = (per + 3) / 4;
+  const long shared = a.c.batch + (kSlots + per - 1) / per;
+  const long apart = a.c.batch + (2 * kSlots + own - 1) / own;
+  const long blocks = max(w.apart ? 0 : shared * per, apart * own);
   if (blocks > 0x7fffffffL)
     throw std::runtime_error("paged_decode: too many sequences and heads");
-  const dim3 grid((unsigned)blocks);
-  if (w.waves == 1) k_paged_decode<T, D, 1><<<grid, 256, 0, stream>>>(a, w);
-  else k_paged_decode<T, D, 4><<<grid, 256, 0, stream>>>(a, w);
+  k_paged_decode<T, D><<<dim3((unsigned)blocks), 256, 0, stream>>>(a, w);
   launched("paged_decode");
   // nothing to join where no sequence can have two chunks
   const int spans = a.mass ? (a.c.room() + kSpan - 1) / kSpan : 0;
   if (spans || a.c.room() > w.least * kStep) {
-    const dim3 finish(a.c.batch, a.c.kvh, a.qh / a.c.kvh + spans);
-    k_decode_finish<T, D><<<finish, 256, 0, stream>>>(a, w);
+    const dim3 finish(a.c.batch, a.c.kvh, w.joins + spans);
+    k_decode_finish<T, D><<<finish, 64 * kSpanWaves, 0, stream>>>(a, w);
     launched("paged_decode");
   }
 }
 
 void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
   if (!a.c.batch) return;
-  if (a.c.kvh > 65535 || a.qh / a.c.kvh + a.c.room() / kSpan > 65534)
+  if (a.c.kvh > 65535 || a.c.room() / kSpan > 65000)
     throw std::runtime_error("paged_decode: 65535 key heads and 2^25 slots of "
                              "a sequence at most");
   DecodeWork w = decode_work(a.c.batch, a.qh, a.c.kvh);
   w.part = (float *)a.ws;
-  const size_t chunks = 2 * (size_t)w.target + a.c.batch;
+  const size_t chunks = decode_chunks(a.c.batch, a.c.kvh, w);
   w.sum = w.part + chunks * a.qh * a.c.d;
   w.plan = (int *)(w.sum + chunks * a.qh);
   w.logits = a.mass ? (float *)(w.plan + 2 * (size_t)a.c.batch) : nullptr;
