@@ -160,6 +160,11 @@ PACKED = {
     "strided": dict(lens=[90, 20], qh=4, kvh=2, d=128, strided=True),
     "int64": dict(lens=[9, 80], qh=2, kvh=1, d=64, index=torch.int64,
                   prefix=[3, 200]),
+    "wild": dict(lens=[100, 33, 257], qh=4, kvh=2, d=64, wild=True),
+    "wild_16": dict(lens=[70, 200], qh=3, kvh=1, d=128, wild=True,
+                    dtype=torch.float16, prefix=[65, 20], slopes=True),
+    "wild_other": dict(lens=[90, 40], keys=[30, 120], qh=2, kvh=1, d=128,
+                       wild=True, softcap=7.0),
     "many": dict(lens=[(i * 29) % 7 for i in range(150)], qh=2, kvh=1, d=64),
 }
 
@@ -192,6 +197,13 @@ def packed_inputs(name):
         k = normal(gen, (nkeys, kvh, d), dtype)
         v = normal(gen, (nkeys, kvh, d), dtype)
     kcu = kw.get("cu_seqlens_k", cu)
+    if c.get("wild"):  # late keys of each document, which few queries see
+        for e in kcu[1:].tolist():
+            k[e - 1, :, ::3] = BAD[0]
+            v[e - 1] = BAD[0]
+            v[e - 5, :, ::2] = BAD[1]
+            v[e - 5, :, 1::4] = BAD[2]
+            v[e - 20, -1, 3] = BAD[2]
     for t in (k, v):  # rows of no document hold no numbers
         t[:int(kcu[0])] = BAD[0]
         t[int(kcu[-1]):] = BAD[1]

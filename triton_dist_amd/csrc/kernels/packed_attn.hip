@@ -62,6 +62,14 @@ TD_DEV s16x4 read_transposed(const void *lds) {
 template <int D> constexpr int kRowK = D + 8;
 template <int D> constexpr int kRowV = D + 32;
 
+// Infinite or not a number.
+TD_DEV bool wild(bf16 x) {
+  return (__builtin_bit_cast(unsigned short, x) & 0x7f80) == 0x7f80;
+}
+TD_DEV bool wild(_Float16 x) {
+  return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
+}
+
 struct Doc {
   long q0, k0;
   int m, n;   // rows, keys
@@ -131,7 +139,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   constexpr int kLoads = kKeys * kP / (64 * kWaves);
   __shared__ __attribute__((aligned(16))) T lds_k[2][kKeys * kRowK<D>];
   __shared__ __attribute__((aligned(16))) T lds_v[2][kKeys * kRowV<D>];
-  __shared__ int lds_see[kWaves];
+  __shared__ int lds_see[kWaves], lds_all[kWaves], lds_wild;
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int c = lane & 31, h = lane >> 5;
@@ -168,7 +176,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   }
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
-  if (lane == 0) lds_see[wave] = most;
+  if (lane == 0) lds_see[wave] = most, lds_all[wave] = live ? least : doc.n;
+  if (tid == 0) lds_wild = 0;
 
   // A negative scale turns the queries' sign, so that maxima stay maxima; a
   // scale of zero clears them, so that a hidden key's -inf stays one.
@@ -202,9 +211,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   // an instruction takes one scalar register: leave it to these
   asm("" : "+v"(cf));
   __syncthreads();
-  int see = 0;
+  int see = 0, all_see = doc.n;  // keys that some row and that all rows see
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) see = max(see, lds_see[w]);
+  for (int w = 0; w < kWaves; ++w) {
+    see = max(see, lds_see[w]);
+    all_see = min(all_see, lds_all[w]);
+  }
   const int steps = (see + kKeys - 1) / kKeys;
 
   // Keys past the document repeat its last one: their weights are zero.
@@ -230,10 +242,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
       *(vec8<T> *)&lds_k[buf][r * kRowK<D> + piece * 8] = nk[i];
     }
   };
-  auto stage_v = [&](int buf) {
+  // A weight of zero does not hide a value that is no number, so where some
+  // row does not see some key such values are staged as zeros, and added to
+  // the rows that see them at the end.
+  auto some_hidden = [&](int step) { return (step + 1) * kKeys > all_see; };
+  auto stage_v = [&](int step) {
+    const int buf = step & 1;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int r = i * kPer + srow;
+      if (some_hidden(step)) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (wild(nv[i][e])) any = true, nv[i][e] = (T)0.f;
+        if (any) lds_wild = 1;
+      }
       *(vec8<T> *)&lds_v[buf][r * kRowV<D> + piece * 8] = nv[i];
     }
   };
@@ -382,7 +406,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
     __syncthreads();  // this step is there, the other buffers are free
     if (step + 1 < steps) {
       stage_k((step & 1) ^ 1);
-      stage_v((step & 1) ^ 1);
+      stage_v(step + 1);
       fetch(nk, kfrom, a.k_tok, base + 2 * kKeys + 32);
       fetch(nv, vfrom, a.v_tok, base + 2 * kKeys);
     }
@@ -391,6 +415,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
       if (base + 32 < most) work(sb, sa, step, 1);
     }
   }
+  __syncthreads();
+  if (lds_wild)
+    for (int key = all_see / kKeys * kKeys; key < see; ++key) {
+      if (key >= lim) continue;
+      const T *v = (const T *)a.v + (doc.k0 + key) * a.v_tok +
+                   kh * a.v_head + 4 * h;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const T x = v[32 * t + 8 * (r / 4) + r % 4];
+          if (wild(x)) acc[t][r] += (float)x;
+        }
+    }
   if (!live || row0 + c >= doc.m) return;
   l += __shfl_xor(l, 32);
   const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -478,8 +478,7 @@ def flash_prefill_packed_op(q: torch.Tensor, k: torch.Tensor,
     exponentials [T, qh] fp32. A row that sees no key gets zeros and -inf.
     Rows that belong to no document are left as they were in a given `out`,
     and are zeros and -inf in tensors that the call makes (a `lse` always).
-    Keys and values of rows that a document's mask hides from part of its
-    queries have to be finite.
+    What the mask hides from a query does not count, whatever it holds.
     """
     dev, dtype = q.device, q.dtype
     if q.dim() != 3 or k.dim() != 3:
@@ -568,13 +567,19 @@ def _packed_cpu(q, k, v, cu_q, cu_k, causal, prefix, scale, softcap, slopes,
         j = torch.arange(n)
         if slopes is not None:
             s = s - slopes.view(kvh, -1, 1, 1) * (at - j).abs().float()
+        seen = torch.ones(m, n, dtype=torch.bool)
         if causal:
             seen = j <= at
             if prefix is not None:
                 seen = seen | (j < int(prefix[i]))
             s = s.masked_fill(~seen, float("-inf"))
         w, total = _weights_cpu(s)
-        o = torch.matmul(w, v[k0:k0 + n].float().transpose(0, 1)[:, None])
+        vf = v[k0:k0 + n].float().transpose(0, 1)   # [kvh, n, d]
+        wild = ~torch.isfinite(vf)
+        o = torch.matmul(w, torch.where(wild, 0.0, vf)[:, None])
+        for key in wild.any(-1).any(0).nonzero()[:, 0].tolist():
+            o[:, :, seen[:, key]] += torch.where(
+                wild[:, key], vf[:, key], 0.0)[:, None, None]
         out[q0:q1] = o.permute(2, 0, 1, 3).reshape(m, qh, d).to(out.dtype)
         if lse is not None:
             lse[q0:q1] = total.permute(2, 0, 1).reshape(m, qh)
