@@ -321,3 +321,12 @@ def test_captured_prefill_follows_its_lengths():
         assert _same(out, eager)
         want = oracle.packed(q, k, v, starts, prefix=pre)
         oracle.check("out", out, want["out"])
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("weights", [False, True])
+def test_cache_steps(weights, graph):
+    """A PagedKVCache through prompts, steps and cuts."""
+    import paged_cache_loop
+
+    paged_cache_loop.run("cuda", weights, graph)

@@ -187,3 +187,20 @@ def test_append_refuses():
             (k, dict(pos=torch.tensor([0, 2])), "both")]:
         with pytest.raises(ValueError, match=words):
             ops.paged_append_op(new, new, *at, **kw)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_cache_steps(weights):
+    import paged_cache_loop
+
+    paged_cache_loop.run("cpu", weights)
+
+
+def test_cache_refuses():
+    from triton_dist_amd.models import PagedKVCache
+
+    cache = PagedKVCache(1, 2, 64, 2, 64, block=16)
+    with pytest.raises(RuntimeError, match="without weights"):
+        cache.evict(8, 2)
+    with pytest.raises(ValueError, match="reserve"):
+        cache.reserve(65)

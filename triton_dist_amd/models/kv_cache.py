@@ -58,14 +58,18 @@ class PagedKVCache:
     blocks allocated on first touch. Serving engines get allocation at
     block granularity instead of max_len * batch up front.
 
-    The HIP decode kernels consume contiguous [B, L, kvh, D];
-    `gather_layer` materializes that view from the table (a functional
-    bridge — a natively paged flash-decode indexing the table in-kernel
-    is roadmap)."""
+    `gather_layer` materializes a contiguous [B, L, kvh, D] view for the
+    kernels that want one. A decode step reads the pages themselves: after
+    `reserve` has handed out pages, `begin_step`, for every layer `write`
+    and `attend`, then `end_step`, all of it without the host and for
+    sequences of unlike lengths, so that a step can be captured. With
+    `weights` the cache also keeps the attention weight that each slot got
+    and each slot's position, and `evict` cuts it to a budget by them."""
 
     def __init__(self, n_layers: int, batch: int, max_len: int,
                  n_kv_heads: int, head_dim: int, block: int = 64,
-                 n_blocks: int = 0, device="cpu", dtype=torch.bfloat16):
+                 n_blocks: int = 0, device="cpu", dtype=torch.bfloat16,
+                 weights: bool = False):
         assert max_len % block == 0
         self.n_layers, self.batch = n_layers, batch
         self.max_len, self.block = max_len, block
@@ -83,11 +87,96 @@ class PagedKVCache:
                                       dtype=torch.int64, device=device)
         self.seq_len = torch.zeros(batch, dtype=torch.int64, device=device)
         self._free_top = 0
+        # of the step under way: its tokens, and the lengths with them
+        self._count = torch.ones_like(self.seq_len)
+        self._live = torch.zeros_like(self.seq_len)
+        # the position of a sequence's next token, which eviction leaves
+        self.next_pos = torch.zeros_like(self.seq_len)
+        self.mass = self.key_pos = None
+        if weights:
+            plane = (n_layers, batch, n_kv_heads, max_len)
+            self.mass = torch.zeros(plane, device=device)
+            self.key_pos = torch.full(plane, -1, device=device,
+                                      dtype=torch.int32)
 
     def reset(self):
         self.block_table.fill_(-1)
         self.seq_len.zero_()
+        self.next_pos.zero_()
         self._free_top = 0
+        if self.mass is not None:
+            self.mass.zero_()
+            self.key_pos.fill_(-1)
+
+    # ------------------------------------------------- steps over the pages
+    def reserve(self, upto_len: int):
+        """Hand out pages for every sequence up to `upto_len` slots (on the
+        host: once, outside of a captured step)."""
+        if upto_len > self.max_len:
+            raise ValueError(f"reserve: {upto_len} of {self.max_len} slots")
+        self._ensure_blocks(upto_len)
+
+    def begin_step(self, counts=1):
+        """A step that adds `counts` tokens to the sequences: one number, or
+        [B] of them."""
+        if isinstance(counts, torch.Tensor):
+            self._count.copy_(counts)
+        else:
+            self._count.fill_(counts)
+        torch.add(self.seq_len, self._count, out=self._live)
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor,
+              cu_seqlens: "torch.Tensor | None" = None):
+        """The step's keys and values: [B, kvh, D] with one token a
+        sequence, or packed [T, kvh, D] with `cu_seqlens` [B + 1]."""
+        from ..ops.paged import paged_append_op
+
+        key_pos = pos = None
+        if self.mass is not None:
+            key_pos, pos = self.key_pos[layer], self.next_pos
+            if cu_seqlens is not None:
+                at = torch.arange(k.shape[0], device=k.device)
+                cu = cu_seqlens.to(torch.int64)
+                seq = torch.searchsorted(cu[1:].contiguous(), at, right=True)
+                seq.clamp_(max=self.batch - 1)
+                pos = pos[seq] + at - cu[seq]
+        paged_append_op(k, v, self.k_pool[layer], self.v_pool[layer],
+                        self.block_table, self.seq_len,
+                        cu_seqlens=cu_seqlens, key_pos=key_pos, pos=pos)
+
+    def attend(self, layer: int, q: torch.Tensor, **score) -> torch.Tensor:
+        """Attention of the step's last token of each sequence, q [B, qh, D]
+        to [B, qh, D], over the slots with the step's own. `score`: scale,
+        softcap and slopes of `paged_decode_op`."""
+        from ..ops.paged import paged_decode_op
+
+        at = (q, self.k_pool[layer], self.v_pool[layer], self.block_table,
+              self._live)
+        if self.mass is None:
+            return paged_decode_op(*at, **score)
+        last = self.next_pos + self._count - 1
+        return paged_decode_op(*at, key_pos=self.key_pos[layer], q_pos=last,
+                               mass=self.mass[layer],
+                               mass_out=self.mass[layer], **score)[0]
+
+    def end_step(self):
+        self.seq_len.copy_(self._live)
+        self.next_pos.add_(self._count)
+
+    def evict(self, budget: int, recent: int):
+        """Between steps: cut every sequence to `budget` slots, in every
+        layer and for every key head by its own weights (`kv_evict_op`)."""
+        from ..ops.paged import kv_evict_op
+
+        if self.mass is None:
+            raise RuntimeError("PagedKVCache.evict: made without weights")
+        for layer in range(self.n_layers):
+            kv_evict_op(self.k_pool[layer], self.v_pool[layer],
+                        self.block_table, self.seq_len, self.mass[layer],
+                        self.key_pos[layer], budget, recent,
+                        out=(self._live, self.mass[layer],
+                             self.key_pos[layer]))
+        self.seq_len.copy_(self._live)
 
     def _ensure_blocks(self, upto_len: int):
         """Allocate pool blocks for every sequence up to `upto_len`
