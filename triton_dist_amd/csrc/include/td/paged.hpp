@@ -48,6 +48,40 @@ struct PagedArgs {
   }
 };
 
+// Of all lanes, to all lanes: lane i takes from lanes 1, 2, 4 and 8 before it
+// in its row of 16, then rows 1 and 3 from the row before, then 2 and 3 from
+// lane 31, which leaves the whole in lane 63.
+#define TD_WAVE_STEPS(X) \
+  X(0x111, 0xf) X(0x112, 0xf) X(0x114, 0xf) X(0x118, 0xf) X(0x142, 0xa) \
+  X(0x143, 0xc)
+TD_DEV float wave_max(float x) {
+#define TD_STEP(ctrl, rows)                                                 \
+  x = fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(                 \
+                   __float_as_uint(x), __float_as_uint(x), ctrl, rows, 0xf, \
+                   false)));
+  TD_WAVE_STEPS(TD_STEP)
+#undef TD_STEP
+  return __uint_as_float(
+      __builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+TD_DEV float wave_sum(float x) {
+#define TD_STEP(ctrl, rows)                                             \
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(                     \
+      0, __float_as_uint(x), ctrl, rows, 0xf, true));
+  TD_WAVE_STEPS(TD_STEP)
+#undef TD_STEP
+  return __uint_as_float(
+      __builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+// Sums over the lanes up to and with this one.
+TD_DEV int wave_scan(int x) {
+#define TD_STEP(ctrl, rows) \
+  x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, true);
+  TD_WAVE_STEPS(TD_STEP)
+#undef TD_STEP
+  return x;
+}
+
 // How a score becomes a logit: capped by a tanh, then lowered by the
 // distance between the query's and the key's position.
 struct ScoreArgs {

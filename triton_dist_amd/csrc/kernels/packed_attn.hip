@@ -18,8 +18,8 @@
 // 8 (r / 4) + 4 h + r % 4, r = 0..15, so maxima and sums need one exchange
 // with the other half of the wave, and those scores are just what the second
 // product wants from this lane once its keys are numbered that way: the
-// weights never leave the registers. K and V come as they lie, by direct
-// loads to LDS, 64 keys a step and two steps deep; V is read transposed.
+// weights never leave the registers. K and V go through registers to LDS,
+// 64 keys a step; V is read transposed.
 #include <stdexcept>
 #include <string>
 
@@ -71,10 +71,10 @@ TD_DEV bool wild(_Float16 x) {
 }
 
 struct Doc {
-  long q0, k0;
-  int m, n;   // rows, keys
-  int index;
-  int block;  // the workgroup's number in the document, from its end
+  int q0, k0;  // first row, first key
+  int m, n;    // rows, keys
+  int prefix;  // keys that all rows see
+  int block;   // the workgroup's number in the document, from its end
 };
 
 // The document's workgroup `at`, or what is left of `at` where there is
@@ -83,30 +83,29 @@ TD_DEV bool find_doc(const PackedArgs &a, int &at, Doc &out) {
   const int lane = threadIdx.x & 63, g = a.qh / a.kvh;
   for (int base = 0; base < a.seqs; base += 64) {
     const int i = base + lane;
-    long q0 = 0;
-    int m = 0, blocks = 0;
-    if (i < a.seqs) {
-      q0 = min(max(a.cu_q[i], 0L), a.rows);
-      m = (int)(min(max(a.cu_q[i + 1], q0), a.rows) - q0);
-      blocks = (int)(((long)((m + kRows - 1) / kRows) * g + kWaves - 1) /
+    int q0 = 0, k0 = 0, m = 0, n = 0, prefix = 0, blocks = 0;
+    if (i < a.seqs) {  // all loads at once: each takes as long as a scan
+      const long q1 = a.cu_q[i + 1], k1 = a.cu_k[i + 1];
+      q0 = (int)min(max(a.cu_q[i], 0L), a.rows);
+      k0 = (int)min(max(a.cu_k[i], 0L), a.keys);
+      if (a.causal && a.prefix.p)
+        prefix = (int)min(max(a.prefix[i], 0L), a.keys);
+      m = (int)min(max(q1, (long)q0), a.rows) - q0;
+      n = (int)min(max(k1, (long)k0), a.keys) - k0;
+      blocks = (int)(((long)((m + kRows - 1L) / kRows) * g + kWaves - 1) /
                      kWaves);
     }
-    int upto = blocks;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o);
-      if (lane >= o) upto += x;
-    }
+    const int upto = wave_scan(blocks);
     const unsigned long long found = __ballot(upto > at);
     if (found) {
       const int f = __builtin_ctzll(found);
-      out.index = base + f;
       // heavy blocks, which see most keys, first
       out.block = __builtin_amdgcn_readlane(upto, f) - 1 - at;
+      out.q0 = __builtin_amdgcn_readlane(q0, f);
+      out.k0 = __builtin_amdgcn_readlane(k0, f);
       out.m = __builtin_amdgcn_readlane(m, f);
-      out.q0 = min(max(a.cu_q[out.index], 0L), a.rows);
-      out.k0 = min(max(a.cu_k[out.index], 0L), a.keys);
-      out.n = (int)(min(max(a.cu_k[out.index + 1], out.k0), a.keys) -
-                    out.k0);
+      out.n = __builtin_amdgcn_readlane(n, f);
+      out.prefix = __builtin_amdgcn_readlane(prefix, f);
       return true;
     }
     at -= __builtin_amdgcn_readlane(upto, 63);
@@ -137,8 +136,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
     PackedArgs a, int tiles) {
   constexpr int kP = D / 8;          // 16-byte pieces of a row
   constexpr int kLoads = kKeys * kP / (64 * kWaves);
-  __shared__ __attribute__((aligned(16))) T lds_k[2][kKeys * kRowK<D>];
-  __shared__ __attribute__((aligned(16))) T lds_v[2][kKeys * kRowV<D>];
+  constexpr int kStageK = kKeys * kRowK<D>, kStageV = kKeys * kRowV<D>;
+  __shared__ __attribute__((aligned(16))) T stage_lds[2 * (kStageK + kStageV)];
+  T *const lds_k = stage_lds, *const lds_v = stage_lds + 2 * kStageK;
   __shared__ int lds_see[kWaves], lds_all[kWaves], lds_wild;
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -151,19 +151,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
       clear_tail<T>(a, at, tiles - ((int)(blockIdx.x / a.kvh) - at), kh);
     return;
   }
+  // Keys past the document repeat its last one: their weights are zero.
+  constexpr int kPer = 64 * kWaves / kP;  // rows that the workgroup moves
+  const int srow = tid / kP, piece = tid % kP;
+  const T *kfrom = (const T *)a.k + (long)doc.k0 * a.k_tok + kh * a.k_head +
+                   piece * 8;
+  const T *vfrom = (const T *)a.v + (long)doc.k0 * a.v_tok + kh * a.v_head +
+                   piece * 8;
+  vec8<T> nk[kLoads], nv[kLoads];
+  int see = doc.n;  // keys that some row sees
+  auto fetch = [&](vec8<T> *to, const T *from, long tok, int first) {
+    if (see <= 0 || first >= see) return;  // also a document without keys
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = max(0, min(first + i * kPer + srow, doc.n - 1));
+      to[i] = *(const vec8<T> *)(from + (long)key * tok);
+    }
+  };
+  vec8<T> after[kLoads];
+  fetch(nk, kfrom, a.k_tok, -32);
+  fetch(after, kfrom, a.k_tok, 32);
+  fetch(nv, vfrom, a.v_tok, 0);
+
   const int units = (doc.m + kRows - 1) / kRows * g;
   const int unit = doc.block * kWaves + wave;
   const bool live = unit < units;
   const int head = kh * g + (live ? unit % g : 0);
   const int row0 = live ? unit / g * kRows : 0;
   const int row = min(row0 + c, doc.m - 1);  // a last unit repeats its last
+  vec8<T> qf[D / 16];
+  {
+    const T *q = (const T *)a.q + (long)(doc.q0 + row) * a.q_tok +
+                 head * a.q_head + h * 8;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) qf[s] = *(const vec8<T> *)(q + s * 16);
+  }
   // keys that this row sees: those below `lim`
   const int pos = row + doc.n - doc.m;
   int lim = doc.n;
   if (a.causal) {
-    lim = min(max(pos + 1, 0), doc.n);
-    if (a.prefix.p)
-      lim = max(lim, (int)min(a.prefix[doc.index], (long)doc.n));
+    lim = max(min(max(pos + 1, 0), doc.n), min(doc.prefix, doc.n));
   }
   if (!live) lim = 0;
   const bool only_back = a.causal && !a.prefix.p;
@@ -179,20 +206,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   if (lane == 0) lds_see[wave] = most, lds_all[wave] = live ? least : doc.n;
   if (tid == 0) lds_wild = 0;
 
-  // A negative scale turns the queries' sign, so that maxima stay maxima; a
-  // scale of zero clears them, so that a hidden key's -inf stays one.
   const float c1 = (a.s.scale == 0.f ? 1.f : fabsf(a.s.scale)) * kLog2e;
-  vec8<T> qf[D / 16];
-  {
-    const T *q = (const T *)a.q + (doc.q0 + row) * a.q_tok +
-                 head * a.q_head + h * 8;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      qf[s] = *(const vec8<T> *)(q + s * 16);
-      if (a.s.scale < 0.f) qf[s] = -qf[s];
-      if (a.s.scale == 0.f) qf[s] = vec8<T>{};
-    }
-  }
   // A logit in units of log2 is cf x + c0, less slope times the distance:
   // x is the score itself, or with a cap 1 / (1 + e^(2 s / cap)), of which
   // cap tanh is cap - 2 cap x.
@@ -211,7 +225,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   // an instruction takes one scalar register: leave it to these
   asm("" : "+v"(cf));
   __syncthreads();
-  int see = 0, all_see = doc.n;  // keys that some row and that all rows see
+  see = 0;
+  int all_see = doc.n;  // keys that all rows see
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     see = max(see, lds_see[w]);
@@ -219,27 +234,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   }
   const int steps = (see + kKeys - 1) / kKeys;
 
-  // Keys past the document repeat its last one: their weights are zero.
-  constexpr int kPer = 64 * kWaves / kP;  // rows that the workgroup moves
-  const int srow = tid / kP, piece = tid % kP;
-  const T *kfrom = (const T *)a.k + doc.k0 * a.k_tok + kh * a.k_head +
-                   piece * 8;
-  const T *vfrom = (const T *)a.v + doc.k0 * a.v_tok + kh * a.v_head +
-                   piece * 8;
-  vec8<T> nk[kLoads], nv[kLoads];
-  auto fetch = [&](vec8<T> *to, const T *from, long tok, int first) {
-    if (first >= see) return;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int key = max(0, min(first + i * kPer + srow, doc.n - 1));
-      to[i] = *(const vec8<T> *)(from + key * tok);
-    }
-  };
-  auto stage_k = [&](int buf) {
+  auto stage_k = [&](const vec8<T> *from, int buf) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int r = i * kPer + srow;
-      *(vec8<T> *)&lds_k[buf][r * kRowK<D> + piece * 8] = nk[i];
+      *(vec8<T> *)&lds_k[buf * kStageK + r * kRowK<D> + piece * 8] = from[i];
     }
   };
   // A weight of zero does not hide a value that is no number, so where some
@@ -258,7 +257,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
           if (wild(nv[i][e])) any = true, nv[i][e] = (T)0.f;
         if (any) lds_wild = 1;
       }
-      *(vec8<T> *)&lds_v[buf][r * kRowV<D> + piece * 8] = nv[i];
+      *(vec8<T> *)&lds_v[buf * kStageV + r * kRowV<D> + piece * 8] = nv[i];
     }
   };
 
@@ -268,13 +267,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   const int vread = (4 * h + ((lane & 15) >> 2)) * kRowV<D> + (lane & 16) +
                     4 * (lane & 3);
   auto k_frag = [&](int buf, int sub, int x) {
-    return *(const vec8<T> *)(&lds_k[0][buf * kKeys * kRowK<D> + kread +
+    return *(const vec8<T> *)(&lds_k[buf * kStageK + kread +
                                         32 * sub * kRowK<D> + 16 * x]);
   };
   auto v_frag = [&](int buf, int sub, int j) {
     constexpr int n = D / 32;
     union { s16x4 half[2]; vec8<T> all; } v;
-    const T *at = &lds_v[0][buf * kKeys * kRowV<D> + vread +
+    const T *at = &lds_v[buf * kStageV + vread +
                             (32 * sub + 16 * (j / n)) * kRowV<D> +
                             32 * (j % n)];
     v.half[0] = read_transposed(at);
@@ -378,15 +377,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   // products made in it, 32 keys further.
   f32x16 sa, sb;
   if (steps) {
-    fetch(nk, kfrom, a.k_tok, -32);
-    fetch(nv, vfrom, a.v_tok, 0);
-    stage_k(1);
+    stage_k(nk, 1);
+    stage_k(after, 0);
     stage_v(0);
-    fetch(nk, kfrom, a.k_tok, 32);
-    stage_k(0);
     fetch(nk, kfrom, a.k_tok, kKeys + 32);
     fetch(nv, vfrom, a.v_tok, kKeys);
     __syncthreads();
+    // A negative scale turns the queries' sign, so that maxima stay maxima;
+    // a scale of zero clears them, so that a hidden key's -inf stays one.
+    if (!(a.s.scale > 0.f))
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x)
+        qf[x] = a.s.scale < 0.f ? -qf[x] : vec8<T>{};
     if (most > 0) {
 #pragma unroll
       for (int x = 0; x < D / 16; ++x)
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
     const int base = step * kKeys;
     __syncthreads();  // this step is there, the other buffers are free
     if (step + 1 < steps) {
-      stage_k((step & 1) ^ 1);
+      stage_k(nk, (step & 1) ^ 1);
       stage_v(step + 1);
       fetch(nk, kfrom, a.k_tok, base + 2 * kKeys + 32);
       fetch(nv, vfrom, a.v_tok, base + 2 * kKeys);
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   if (lds_wild)
     for (int key = all_see / kKeys * kKeys; key < see; ++key) {
       if (key >= lim) continue;
-      const T *v = (const T *)a.v + (doc.k0 + key) * a.v_tok +
+      const T *v = (const T *)a.v + (long)(doc.k0 + key) * a.v_tok +
                    kh * a.v_head + 4 * h;
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
@@ -429,11 +431,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
           if (wild(x)) acc[t][r] += (float)x;
         }
     }
-  if (!live || row0 + c >= doc.m) return;
   l += __shfl_xor(l, 32);
+  if (!live) return;
+  if (a.lse && h == 0 && row0 + c < doc.m)
+    a.lse[(long)(doc.q0 + row) * a.qh + head] =
+        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  // Through LDS, where nothing is read any more, so that whole rows go out.
+  constexpr int kRowO = D + 8;
+  static_assert(kWaves * kRows * kRowO <= 2 * (kStageK + kStageV),
+                "outputs fit where K and V were");
+  T *mine = &stage_lds[wave * kRows * kRowO];
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *out = (T *)a.out + (doc.q0 + row) * a.out_tok + head * a.out_head +
-           4 * h;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -441,11 +449,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
       vec4<T> o;
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = (T)(acc[t][r + i] * inv);
-      *(vec4<T> *)(out + 32 * t + 2 * r) = o;
+      *(vec4<T> *)(mine + c * kRowO + 32 * t + 2 * r + 4 * h) = o;
     }
-  if (a.lse && h == 0)
-    a.lse[(doc.q0 + row) * a.qh + head] =
-        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+  T *out = (T *)a.out + (long)(doc.q0 + row0) * a.out_tok + head * a.out_head;
+#pragma unroll
+  for (int i = 0; i < kRows * kP / 64; ++i) {
+    const int r = (i * 64 + lane) / kP, e = lane % kP * 8;
+    if (row0 + r < doc.m)
+      *(vec8<T> *)(out + r * a.out_tok + e) =
+          *(const vec8<T> *)(mine + r * kRowO + e);
+  }
 }
 
 template <typename T, int D>
@@ -472,6 +487,8 @@ void prefill(const PackedArgs &a, hipStream_t stream) {
 
 void launch_packed_prefill(const PackedArgs &a, hipStream_t stream) {
   if (!a.rows) return;
+  if (a.rows > 0x7fffffffL || a.keys > 0x7fffffffL)
+    throw std::runtime_error("packed_prefill: too many rows");
   if (a.is_fp16)
     a.d == 64 ? prefill<_Float16, 64>(a, stream)
               : prefill<_Float16, 128>(a, stream);
