@@ -6,10 +6,10 @@
 // pair, against a few bytes per token. One pass over the keys with running
 // maxima and sums.
 //
-// A wave owns a unit: 32 rows of one query head. The eight units of a
-// workgroup share one key head's K and V, and units are numbered heads
-// first, so that with eight query heads to a key head a workgroup's units
-// are the same 32 rows: they need the same keys, and the causal boundary
+// A wave owns a unit: 32 rows of one query head. The units of a workgroup
+// share one key head's K and V, and units are numbered heads first, so that
+// with eight query heads to a key head a workgroup's units are the same 32
+// rows: they need the same keys, and the causal boundary
 // costs one partly seen tile. Any number of query heads per key head packs
 // without a gap.
 //
@@ -38,7 +38,12 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kWaves = 8, kRows = 32, kKeys = 64;
+constexpr int kRows = 32, kKeys = 64;
+// Of a workgroup. With rows of 64 elements more of a step's work is vector
+// instructions, and two workgroups of four on a SIMD's waves overlap better
+// (16384 tokens, capped: 1.70 ms for 1.90); with 128 sharing K and V among
+// eight does (plain: 2.32 ms for 2.43).
+template <int D> constexpr int kWavesOf = D == 64 ? 4 : 8;
 // A maximum may fall behind by this many powers of two before the sums are
 // rescaled: weights up to 2^6 cost no precision.
 constexpr float kSlack = 6.f;
@@ -79,7 +84,9 @@ struct Doc {
 
 // The document's workgroup `at`, or what is left of `at` where there is
 // none: the number of the workgroup among the spare ones.
+template <int D>
 TD_DEV bool find_doc(const PackedArgs &a, int &at, Doc &out) {
+  constexpr int kWaves = kWavesOf<D>;
   const int lane = threadIdx.x & 63, g = a.qh / a.kvh;
   for (int base = 0; base < a.seqs; base += 64) {
     const int i = base + lane;
@@ -132,8 +139,9 @@ TD_DEV void clear_tail(const PackedArgs &a, int spare, int spares, int kh) {
 }
 
 template <typename T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
+__global__ __launch_bounds__(64 * kWavesOf<D>, 2) void k_packed_prefill(
     PackedArgs a, int tiles) {
+  constexpr int kWaves = kWavesOf<D>;
   constexpr int kP = D / 8;          // 16-byte pieces of a row
   constexpr int kLoads = kKeys * kP / (64 * kWaves);
   constexpr int kStageK = kKeys * kRowK<D>, kStageV = kKeys * kRowV<D>;
@@ -146,7 +154,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_packed_prefill(
   const int kh = blockIdx.x % a.kvh, g = a.qh / a.kvh;
   int at = blockIdx.x / a.kvh;
   Doc doc;
-  if (!find_doc(a, at, doc)) {
+  if (!find_doc<D>(a, at, doc)) {
     if (a.clear_tail || a.lse)  // `at` is past the documents' workgroups
       clear_tail<T>(a, at, tiles - ((int)(blockIdx.x / a.kvh) - at), kh);
     return;
@@ -467,6 +475,7 @@ template <typename T, int D>
 void prefill(const PackedArgs &a, hipStream_t stream) {
   // as many workgroups a key head as any cutting of the rows into documents
   // can need, and spare ones for the rows of no document
+  constexpr int kWaves = kWavesOf<D>;
   const long g = a.qh / a.kvh;
   const long tiles = (a.rows / kRows + a.seqs) * g / kWaves + a.seqs + 4;
   if (tiles * a.kvh > 0x7fffffffL)
