@@ -105,10 +105,13 @@ def test_evict(name, inplace):
 @pytest.mark.parametrize("single", [True, False])
 @pytest.mark.parametrize("heads, d, block", [(2, 16, 8), (5, 128, 7),
                                              (8, 64, 64)])
-def test_append(dtype, single, heads, d, block):
+@pytest.mark.parametrize("tell", [None, [-3, 1 << 40, 5, 80]])
+def test_append(dtype, single, heads, d, block, tell):
     lens = [5, 16, 0, 63]
     st = cases.cache(3, lens, heads, d, block, dtype, extra=11,
                      missing=[(1, 2)])
+    if tell:  # what the lengths' tensor says
+        st["lens"] = torch.tensor(tell)
     gen = st["gen"]
     cu = torch.tensor([2, 2, 9, 10, 21])
     rows = 4 if single else 23

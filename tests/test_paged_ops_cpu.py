@@ -204,3 +204,6 @@ def test_cache_refuses():
         cache.evict(8, 2)
     with pytest.raises(ValueError, match="reserve"):
         cache.reserve(65)
+    cache = PagedKVCache(1, 2, 64, 2, 64, block=16, weights=True)
+    with pytest.raises(RuntimeError, match="by write"):
+        cache.append(0, torch.zeros(2, 1, 2, 64), torch.zeros(2, 1, 2, 64), 0)

@@ -41,11 +41,11 @@ __global__ __launch_bounds__(256) void k_paged_append(
     }
     if (lo >= a.batch || t < cu[lo]) return;
     b = lo;
-    slot = a.lens[b] + t - cu[b];
+    slot = max(a.lens[b], 0L) + t - cu[b];
   } else {
-    slot = a.lens[b];
+    slot = max(a.lens[b], 0L);
   }
-  if (slot < 0 || slot >= a.room()) return;
+  if (slot >= a.room()) return;
   const long page = a.page(b, (int)slot);
   if (page < 0) return;
   const int row = (int)slot % a.block;
@@ -66,13 +66,13 @@ __global__ __launch_bounds__(256) void k_paged_append(
 // key head of one and up to 16 of its query heads, or a quarter of the tiles
 // of that (find_cut).
 //
-// A wave goes through its 32-key tiles without a barrier. S^T = K Q^T and O^T = V^T P^T, so that a lane
-// holds the scores of one query head all the way: lane (n, qd) = (lane & 15,
-// lane >> 4) gets from the 16x16x32 matrix instructions the scores of head n
-// and keys 16 t + 4 qd + i, which are the elements that the second product
-// wants from it, once its 32 keys are numbered (qd, t, i). K goes from
-// global memory to the operand's registers; V takes a way through the
-// wave's piece of LDS, where it is read transposed.
+// A wave goes through its 32-key tiles without a barrier. S^T = K Q^T and
+// O^T = V^T P^T, so that a lane holds the scores of one query head all the
+// way: lane (n, qd) = (lane & 15, lane >> 4) gets from the 16x16x32 matrix
+// instructions the scores of head n and keys 16 t + 4 qd + i, which are the
+// elements that the second product wants from it, once its 32 keys are
+// numbered (qd, t, i). K goes from global memory to the operand's registers;
+// V takes a way through the wave's piece of LDS, where it is read transposed.
 //
 // The weights meet V in the inputs' type, as a rounded part and the rounded
 // rest: the second product is far from bounding the kernel, and with it the
@@ -945,6 +945,8 @@ void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
   if (a.c.kvh > 65535 || a.c.room() / kSpan > 65000)
     throw std::runtime_error("paged_decode: 65535 key heads and 2^25 slots of "
                              "a sequence at most");
+  if ((long)a.c.batch * (a.c.room() / kStep + 1) > 1L << 30)
+    throw std::runtime_error("paged_decode: 2^37 slots in all at most");
   DecodeWork w = decode_work(a.c.batch, a.qh, a.c.kvh);
   w.part = (float *)a.ws;
   const size_t chunks = decode_chunks(a.c.batch, a.c.kvh, w);

@@ -198,6 +198,9 @@ class PagedKVCache:
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor,
                pos0: int):
         """k/v: [B, S, kvh, D] written at positions [pos0, pos0+S)."""
+        if self.mass is not None:
+            raise RuntimeError("PagedKVCache.append: a cache with weights "
+                               "takes its tokens by write")
         b, s = k.shape[0], k.shape[1]
         self._ensure_blocks(pos0 + s)
         for off in range(s):

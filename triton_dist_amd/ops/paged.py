@@ -230,8 +230,8 @@ def paged_append_op(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
                                                   tokens)
         first = lo if cu_seqlens is None else int(cu_seqlens[i])
         for t in range(lo, hi):
-            slot = int(seq_lens[i]) + t - first
-            if not 0 <= slot < room:
+            slot = max(int(seq_lens[i]), 0) + t - first
+            if slot >= room:
                 continue
             page = int(block_table[i, slot // block])
             if not 0 <= page < n:
