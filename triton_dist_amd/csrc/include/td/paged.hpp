@@ -64,6 +64,13 @@ TD_DEV float wave_max(float x) {
   return __uint_as_float(
       __builtin_amdgcn_readlane(__float_as_uint(x), 63));
 }
+TD_DEV int wave_max(int x) {
+#define TD_STEP(ctrl, rows) \
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, ctrl, rows, 0xf, false));
+  TD_WAVE_STEPS(TD_STEP)
+#undef TD_STEP
+  return __builtin_amdgcn_readlane(x, 63);
+}
 TD_DEV float wave_sum(float x) {
 #define TD_STEP(ctrl, rows)                                             \
   x += __uint_as_float(__builtin_amdgcn_update_dpp(                     \

@@ -626,12 +626,14 @@ TD_DEV unsigned rank_key(float mass, bool is_recent) {
 
 constexpr int kEvict = 1024;              // threads, and slots of a pass
 constexpr int kEvictWaves = kEvict / 64;
-constexpr int kPairs = 64;                // rows that a workgroup moves
+constexpr int kPairs = 32;                // rows that a workgroup moves
 
 // What goes where: the i-th free slot below the budget takes the i-th kept
-// row above it. ws: [batch, kvh] counts, then [batch, kvh, pairs] of these.
+// row above it. ws: [batch, kvh, pairs] of these, then [batch, kvh] counts.
 struct Pair {
   int to, from;
+  float mass;  // the moved row's
+  int pos;
 };
 
 // R passes of slots are kept in registers as keys; longer sequences (MANY)
@@ -639,8 +641,8 @@ struct Pair {
 template <int R, bool MANY>
 __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
                                                          int pairs) {
-  __shared__ int lds_n[kEvictWaves], hist[256];
-  __shared__ int lds_c[3][R][kEvictWaves];
+  __shared__ int lds_n[kEvictWaves], hists[4][256];
+  __shared__ int lds_c[2][R][kEvictWaves], lds_all[2];
   const int b = blockIdx.x / a.c.kvh, h = blockIdx.x % a.c.kvh;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int room = a.c.room(), len = a.c.len(b);
@@ -650,9 +652,8 @@ __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
   const int *pos = a.key_pos + row;
   float *mass_out = a.mass_out + row;
   int *pos_out = a.key_pos_out + row;
-  int *count = (int *)a.ws + blockIdx.x;
-  Pair *list = (Pair *)((int *)a.ws + (long)a.c.batch * a.c.kvh) +
-               (long)blockIdx.x * pairs;
+  int *count = (int *)((Pair *)a.ws + (long)gridDim.x * pairs) + blockIdx.x;
+  Pair *list = (Pair *)a.ws + (long)blockIdx.x * pairs;
   if (keep == len) {
     for (int i = tid; i < room; i += kEvict) {
       const float m = i < len ? mass[i] : 0.f;
@@ -664,48 +665,50 @@ __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
     return;
   }
 
+  (&hists[0][0])[tid] = 0;
   // positions from the first one on count as recent
   unsigned key[R];
+  float m[R];
+  int p[R];
   long since = 0;
   constexpr int kPart = R * kEvict;
-  {
-    int newest = INT_MIN, p[R];
-    float m[R];
-    for (int part = 0; part < (MANY ? len : 1); part += kPart)
+  auto read = [&](int part) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int i = part + r * kEvict + tid;
-        p[r] = i < len ? pos[i] : INT_MIN;
-        if (!MANY) m[r] = i < len ? mass[i] : 0.f;
-        newest = max(newest, p[r]);
-      }
-    for (int o = 32; o; o >>= 1) newest = max(newest, __shfl_xor(newest, o));
+    for (int r = 0; r < R; ++r) {
+      const int i = part + r * kEvict + tid;
+      m[r] = i < len ? mass[i] : 0.f;
+      p[r] = i < len ? pos[i] : INT_MIN;
+    }
+  };
+  {
+    int newest = INT_MIN;
+    for (int part = 0; part < (MANY ? len : 1); part += kPart) {
+      read(part);
+#pragma unroll
+      for (int r = 0; r < R; ++r) newest = max(newest, p[r]);
+    }
+    newest = wave_max(newest);
     if (lane == 0) lds_n[wave] = newest;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEvictWaves; ++i) newest = max(newest, lds_n[i]);
     since = (long)newest - a.recent + 1;
-    if (!MANY)
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        key[r] = r * kEvict + tid < len ? rank_key(m[r], p[r] >= since) : 0;
   }
   auto load = [&](int part) {
+    if (MANY) read(part);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int i = part + r * kEvict + tid;
-      key[r] = i < len ? rank_key(mass[i], pos[i] >= since) : 0;
-    }
+    for (int r = 0; r < R; ++r)
+      key[r] = part + r * kEvict + tid < len ? rank_key(m[r], p[r] >= since)
+                                             : 0;
   };
+  if (!MANY) load(0);
 
   // The keep-th largest key, eight bits at a time from the top, by counts of
   // the keys that agree so far. Of those that equal it, `need` stay.
   unsigned t = 0;
   int need = keep;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
+    int *hist = hists[shift / 8];
     for (int part = 0; part < (MANY ? len : 1); part += kPart) {
       if (MANY) load(part);
 #pragma unroll
@@ -747,95 +750,94 @@ __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
     }
   }
 
-  // Ranks in order of the slots, part by part: of the equal ones, of the
-  // free slots below the budget and of the kept rows above it.
-  auto before = [&](int which, int r, int &all) {  // this wave's pass r
-    int sum = 0, own = 0;
-    all = 0;
-    for (int i = lane; i < R * kEvictWaves; i += 64) {
-      const int x = (&lds_c[which][0][0])[i];
-      sum += x;
-      if (i < r * kEvictWaves + wave) own += x;
+  // Ranks in order of the slots, part by part. A wave puts its counts of a
+  // pass into lds_c; `sum_up` makes of them what comes before each.
+  auto sum_up = [&](int which) {
+    __syncthreads();
+    if (wave == 0) {
+      constexpr int kEach = R * kEvictWaves / 64;
+      int *c = &lds_c[which][0][0] + lane * kEach, n[kEach], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += n[i] = c[i];
+      int before = wave_scan(sum) - sum;
+      if (lane == 63) lds_all[which] = before + sum;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) c[i] = before, before += n[i];
     }
-    all = __builtin_amdgcn_readlane(wave_scan(sum), 63);
-    return __builtin_amdgcn_readlane(wave_scan(own), 63);
+    __syncthreads();
   };
   int ties = 0, holes = 0, movers = 0;
   const unsigned long long below = (1ull << lane) - 1;
   for (int part = 0; part < (MANY ? len : 1); part += kPart) {
     if (MANY) load(part);
     unsigned stays = 0;  // bit r
-    if (need) {
-      __syncthreads();
+    if (need) {  // of the equal ones the first stay
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int n = __popcll(__ballot(key[r] == t));
         if (lane == 0) lds_c[0][r][wave] = n;
       }
-      __syncthreads();
+      sum_up(0);
     }
-    int all = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       bool stay = key[r] > t;
-      if (need && __any(key[r] == t)) {
-        const int rank = ties + before(0, r, all) +
-                         __popcll(__ballot(key[r] == t) & below);
+      if (need) {
+        const unsigned long long equal = __ballot(key[r] == t);
+        const int rank = ties + lds_c[0][r][wave] + __popcll(equal & below);
         stay = stay || (key[r] == t && rank < need);
       }
       stays |= (unsigned)stay << r;
     }
     if (need) {
-      before(0, 0, all);
-      ties += all;
+      ties += lds_all[0];
+      __syncthreads();
     }
-    __syncthreads();
+    // free slots below the budget, and kept rows above it
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int i = part + r * kEvict + tid;
       const bool stay = stays >> r & 1;
       const int nh = __popcll(__ballot(i < keep && !stay));
       const int nm = __popcll(__ballot(i >= keep && stay));
-      if (lane == 0) lds_c[1][r][wave] = nh, lds_c[2][r][wave] = nm;
+      if (lane == 0) lds_c[0][r][wave] = nh, lds_c[1][r][wave] = nm;
     }
-    __syncthreads();
-    int all_h, all_m;
-    before(1, 0, all_h);
-    before(2, 0, all_m);
+    sum_up(0);
+    sum_up(1);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int i = part + r * kEvict + tid;
       const bool stay = stays >> r & 1;
       const bool hole = i < keep && !stay, mover = i >= keep && stay;
-      if (__any(hole)) {
-        const int at = holes + before(1, r, all) +
-                       __popcll(__ballot(hole) & below);
-        if (hole) list[at].to = i;
+      const unsigned long long some_h = __ballot(hole);
+      const unsigned long long some_m = __ballot(mover);
+      if (some_h && hole)
+        list[holes + lds_c[0][r][wave] + __popcll(some_h & below)].to = i;
+      if (some_m && mover) {
+        Pair *to = list + movers + lds_c[1][r][wave] +
+                   __popcll(some_m & below);
+        to->from = i;
+        to->mass = m[r];
+        to->pos = p[r];
       }
-      if (__any(mover)) {
-        const int at = movers + before(2, r, all) +
-                       __popcll(__ballot(mover) & below);
-        if (mover) list[at].from = i;
+      if (i < keep && stay) {
+        if (mass_out != mass) mass_out[i] = m[r];
+        if (pos_out != pos) pos_out[i] = p[r];
       }
     }
-    holes += all_h;
-    movers += all_m;
+    holes += lds_all[0];
+    movers += lds_all[1];
+    if (MANY) __syncthreads();
   }
   if (tid == 0) *count = movers;
-  // Bookkeeping. The list is whole, and all of the old is still there.
+  // All of the old has been read, and the list is whole.
   __threadfence_block();
   __syncthreads();
-  if (mass_out != mass)
-    for (int i = tid; i < keep; i += kEvict) mass_out[i] = mass[i];
-  if (pos_out != pos)
-    for (int i = tid; i < keep; i += kEvict) pos_out[i] = pos[i];
-  __syncthreads();
   for (int i = tid; i < movers; i += kEvict) {
-    const Pair p = list[i];
-    mass_out[p.to] = mass[p.from];
-    pos_out[p.to] = pos[p.from];
+    const Pair x = list[i];
+    mass_out[x.to] = x.mass;
+    pos_out[x.to] = x.pos;
   }
-  __syncthreads();
   for (int i = keep + tid; i < room; i += kEvict) {
     mass_out[i] = 0.f;
     pos_out[i] = -1;
@@ -848,15 +850,15 @@ __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
 __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a, int pairs) {
   const int b = blockIdx.x / a.c.kvh, h = blockIdx.x % a.c.kvh;
   const int tid = threadIdx.x;
-  const int n = min(((const int *)a.ws)[blockIdx.x] - (int)blockIdx.y * kPairs,
-                    kPairs);
-  const Pair *list = (const Pair *)((const int *)a.ws +
-                                    (long)a.c.batch * a.c.kvh) +
-                     (long)blockIdx.x * pairs + (long)blockIdx.y * kPairs;
+  const int *count = (const int *)((const Pair *)a.ws +
+                                   (long)gridDim.x * pairs);
+  const int n = min(count[blockIdx.x] - (int)blockIdx.y * kPairs, kPairs);
+  const Pair *list = (const Pair *)a.ws + (long)blockIdx.x * pairs +
+                     (long)blockIdx.y * kPairs;
   const int chunks = a.c.d / 8;
 #pragma unroll 4
   for (int i = tid; i < n * chunks; i += 256) {
-    const Pair p = list[i / chunks];
+    const Pair &p = list[i / chunks];
     const long pt = a.c.page(b, p.to), pf = a.c.page(b, p.from);
     if (pt < 0 || pf < 0) continue;
     const int c = i % chunks * 8;
