@@ -150,6 +150,8 @@ PACKED = {
                       d=64, slopes=True),
     "fewer_keys": dict(lens=[150, 8, 4], keys=[20, 0, 4], qh=2, kvh=1,
                        d=128),
+    "full_prefix": dict(lens=[70, 30], qh=2, kvh=1, d=64, causal=False,
+                        prefix=[20, 0], slopes=True),
     "full_other": dict(lens=[5, 40], keys=[100, 0], qh=2, kvh=1, d=128,
                        causal=False, slopes=True),
     "tail": dict(lens=[40, 9], tail=30, qh=2, kvh=1, d=64),

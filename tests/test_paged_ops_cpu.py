@@ -140,8 +140,6 @@ def _packed_args():
     (dict(at=3, to=lambda t: t[:, None]), "cu_seqlens"),
     (dict(kw=dict(cu_seqlens_k=torch.tensor([0, 9]))), "cu_seqlens"),
     (dict(kw=dict(prefix_lens=torch.tensor([1]))), "prefix_lens"),
-    (dict(kw=dict(prefix_lens=torch.tensor([1, 1]), causal=False)),
-     "prefix_lens"),
     (dict(kw=dict(out=torch.zeros(9, 4, 64))), "out"),
 ])
 def test_packed_refuses(change, words):

@@ -470,7 +470,8 @@ def flash_prefill_packed_op(q: torch.Tensor, k: torch.Tensor,
 
     With `causal`, query i of a document with m queries and n keys sees the
     keys up to i + n - m (the last query sees them all), and besides them
-    the document's first prefix_lens[i] keys. Scores are capped by `softcap`
+    the document's first prefix_lens[i] keys; without it every query sees
+    every key of its document. Scores are capped by `softcap`
     and lowered by `slopes` as in `paged_decode_op`, the distance being that
     from key position i + n - m.
 
@@ -514,8 +515,6 @@ def flash_prefill_packed_op(q: torch.Tensor, k: torch.Tensor,
     else:
         cu_seqlens_k = cu_seqlens
     if prefix_lens is not None:
-        if not causal:
-            _refuse("prefix_lens: without causal every key is seen")
         _array("prefix_lens", prefix_lens, None, (docs,), dev)
     clear = out is None
     if clear:
