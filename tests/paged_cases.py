@@ -168,6 +168,10 @@ PACKED = {
     "wild_other": dict(lens=[90, 40], keys=[30, 120], qh=2, kvh=1, d=128,
                        wild=True, softcap=7.0),
     "many": dict(lens=[(i * 29) % 7 for i in range(150)], qh=2, kvh=1, d=64),
+    "many_128": dict(lens=[(i * 29) % 5 for i in range(80)] + [90], qh=6,
+                     kvh=2, d=128, prefix=[(i * 3) % 4 for i in range(81)]),
+    "very_many": dict(lens=[(i * 29) % 4 for i in range(1300)], qh=1, kvh=1,
+                      d=64, tail=9),
 }
 
 

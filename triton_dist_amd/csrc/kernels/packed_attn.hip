@@ -82,41 +82,80 @@ struct Doc {
   int block;   // the workgroup's number in the document, from its end
 };
 
+// Document i, by offsets that may be anything: nothing outside of the rows
+// and keys comes out. Returns its workgroups.
+template <int D>
+TD_DEV int read_doc(const PackedArgs &a, int i, Doc &out) {
+  const long q0 = a.cu_q[i], q1 = a.cu_q[i + 1], k0 = a.cu_k[i],
+             k1 = a.cu_k[i + 1];  // all loads at once
+  const long prefix = a.causal && a.prefix.p ? a.prefix[i] : 0;
+  out.q0 = (int)min(max(q0, 0L), a.rows);
+  out.k0 = (int)min(max(k0, 0L), a.keys);
+  out.m = (int)min(max(q1, (long)out.q0), a.rows) - out.q0;
+  out.n = (int)min(max(k1, (long)out.k0), a.keys) - out.k0;
+  out.prefix = (int)min(max(prefix, 0L), a.keys);
+  return (int)(((out.m + kRows - 1L) / kRows * (a.qh / a.kvh) +
+                kWavesOf<D> - 1) / kWavesOf<D>);
+}
+
 // The document's workgroup `at`, or what is left of `at` where there is
-// none: the number of the workgroup among the spare ones.
+// none: the number of the workgroup among the spare ones. Heavy workgroups
+// of a document, which see most keys, come first. A wave finds it among up
+// to 64 documents, which needs no barrier; among more the waves share the
+// offsets (16384 tokens, 64 heads of 128, 8 tokens a document: 0.70 ms, and
+// 2.40 where each wave goes through all offsets).
 template <int D>
 TD_DEV bool find_doc(const PackedArgs &a, int &at, Doc &out) {
-  constexpr int kWaves = kWavesOf<D>;
-  const int lane = threadIdx.x & 63, g = a.qh / a.kvh;
-  for (int base = 0; base < a.seqs; base += 64) {
-    const int i = base + lane;
-    int q0 = 0, k0 = 0, m = 0, n = 0, prefix = 0, blocks = 0;
-    if (i < a.seqs) {  // all loads at once: each takes as long as a scan
-      const long q1 = a.cu_q[i + 1], k1 = a.cu_k[i + 1];
-      q0 = (int)min(max(a.cu_q[i], 0L), a.rows);
-      k0 = (int)min(max(a.cu_k[i], 0L), a.keys);
-      if (a.causal && a.prefix.p)
-        prefix = (int)min(max(a.prefix[i], 0L), a.keys);
-      m = (int)min(max(q1, (long)q0), a.rows) - q0;
-      n = (int)min(max(k1, (long)k0), a.keys) - k0;
-      blocks = (int)(((long)((m + kRows - 1L) / kRows) * g + kWaves - 1) /
-                     kWaves);
-    }
+  constexpr int kWaves = kWavesOf<D>, kThreads = 64 * kWaves;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (a.seqs <= 64) {
+    Doc doc{};
+    const int blocks = lane < a.seqs ? read_doc<D>(a, lane, doc) : 0;
     const int upto = wave_scan(blocks);
-    const unsigned long long found = __ballot(upto > at);
+    const unsigned long long found = __ballot(blocks && upto > at);
     if (found) {
       const int f = __builtin_ctzll(found);
-      // heavy blocks, which see most keys, first
       out.block = __builtin_amdgcn_readlane(upto, f) - 1 - at;
-      out.q0 = __builtin_amdgcn_readlane(q0, f);
-      out.k0 = __builtin_amdgcn_readlane(k0, f);
-      out.m = __builtin_amdgcn_readlane(m, f);
-      out.n = __builtin_amdgcn_readlane(n, f);
-      out.prefix = __builtin_amdgcn_readlane(prefix, f);
+      out.q0 = __builtin_amdgcn_readlane(doc.q0, f);
+      out.k0 = __builtin_amdgcn_readlane(doc.k0, f);
+      out.m = __builtin_amdgcn_readlane(doc.m, f);
+      out.n = __builtin_amdgcn_readlane(doc.n, f);
+      out.prefix = __builtin_amdgcn_readlane(doc.prefix, f);
       return true;
     }
     at -= __builtin_amdgcn_readlane(upto, 63);
+    return false;
   }
+  __shared__ int lds_n[kWaves];
+  __shared__ Doc lds_doc;
+  const int each = (a.seqs + kThreads - 1) / kThreads;
+  const int last = min((tid + 1) * each, a.seqs);
+  int own = 0;
+  Doc doc;
+  for (int i = tid * each; i < last; ++i) own += read_doc<D>(a, i, doc);
+  const int upto = wave_scan(own);
+  if (lane == 63) lds_n[wave] = upto;
+  if (tid == 0) lds_doc.m = 0;
+  __syncthreads();
+  int before = upto - own, all = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < wave) before += lds_n[i];
+    all += lds_n[i];
+  }
+  if (at < all && at >= before && at < before + own)
+    for (int i = tid * each; i < last; ++i) {
+      const int blocks = read_doc<D>(a, i, doc);
+      if (at >= before && at < before + blocks) {
+        doc.block = before + blocks - 1 - at;
+        lds_doc = doc;
+      }
+      before += blocks;
+    }
+  __syncthreads();
+  out = lds_doc;
+  if (at < all && out.m > 0) return true;
+  at = max(at - all, 0);
   return false;
 }
 
