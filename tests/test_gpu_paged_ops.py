@@ -132,6 +132,24 @@ def test_append(dtype, single, heads, d, block, tell):
         assert _same(x, y)
 
 
+@pytest.mark.parametrize("first, lens", [
+    (0, [(1 << 63) - 1, 5]), (-(1 << 63), [5, 5]),
+    (-(1 << 63), [(1 << 63) - 1] * 2), (-(1 << 40), [-(1 << 63), 16]),
+    (-3, [-(1 << 63), 16])])
+def test_append_with_any_number(first, lens):
+    """Slots that a sum in 64 bits would turn negative are dropped."""
+    st = cases.cache(8, [5, 16], 2, 64, 8, extra=9)
+    cu = torch.tensor([first, 4, 9])
+    k = cases.normal(st["gen"], (9, 2, 64), torch.bfloat16)
+    lens = torch.tensor(lens)
+    g = _gpu(dict(k=st["k"], v=st["v"], t=st["table"], n=lens, cu=cu, new=k))
+    ops.paged_append_op(k, k, st["k"], st["v"], st["table"], lens,
+                        cu_seqlens=cu)
+    ops.paged_append_op(g["new"], g["new"], g["k"], g["v"], g["t"], g["n"],
+                        cu_seqlens=g["cu"])
+    assert _same(g["k"], st["k"]) and _same(g["v"], st["v"])
+
+
 def test_far_pages_need_64_bits():
     """Pages whose rows start past 2^31 elements."""
     block, kvh, d = 64, 8, 128

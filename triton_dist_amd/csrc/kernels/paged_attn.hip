@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256) void k_paged_append(
   if (t >= tokens) return;
   const int h = (int)(i / chunks % a.kvh), c = (int)(i % chunks);
   int b = (int)t;
-  long slot;
+  unsigned long past = 0;  // slots behind the length; an offset may be anything
   if (cu.p) {
     int lo = 0, hi = a.batch;  // the sequence with cu[b] <= t < cu[b + 1]
     while (lo < hi) {
@@ -41,11 +41,11 @@ __global__ __launch_bounds__(256) void k_paged_append(
     }
     if (lo >= a.batch || t < cu[lo]) return;
     b = lo;
-    slot = max(a.lens[b], 0L) + t - cu[b];
-  } else {
-    slot = max(a.lens[b], 0L);
+    past = (unsigned long)t - (unsigned long)cu[b];
   }
-  if (slot >= a.room()) return;
+  const unsigned long slot = a.len(b) + past;
+  if (past >= (unsigned long)a.room() || slot >= (unsigned long)a.room())
+    return;
   const long page = a.page(b, (int)slot);
   if (page < 0) return;
   const int row = (int)slot % a.block;
