@@ -82,6 +82,9 @@ DECODE = {
                       tell=[1 << 40, -5], mass=True),
     "strong": dict(lens=[400], qh=8, kvh=1, d=128, block=64, std=30.0),
     "no_scale": dict(lens=[50], qh=2, kvh=2, d=64, block=16, scale=0.0),
+    "large_cap": dict(lens=[50, 300], qh=2, kvh=2, d=64, block=16,
+                      softcap=1000.0),
+    "small_cap": dict(lens=[50], qh=2, kvh=2, d=64, block=16, softcap=1e-6),
     "negative": dict(lens=[90, 3], qh=4, kvh=2, d=64, block=16, scale=-0.4),
     "batch": dict(lens=[(i * 37) % 90 for i in range(70)], qh=4, kvh=2,
                   d=64, block=16),
@@ -141,6 +144,8 @@ PACKED = {
     "long_64": dict(lens=[260, 7], qh=2, kvh=1, d=64),
     "full": dict(lens=[70, 130], qh=2, kvh=2, d=64, causal=False),
     "capped": dict(lens=[140], qh=4, kvh=2, d=128, softcap=2.0, std=4.0),
+    "large_cap": dict(lens=[90, 33], qh=2, kvh=1, d=128, softcap=1000.0),
+    "small_cap": dict(lens=[90, 33], qh=2, kvh=1, d=64, softcap=1e-6),
     "sloped": dict(lens=[200, 10], qh=8, kvh=2, d=64, slopes=True),
     "prefix": dict(lens=[150, 5, 90], qh=2, kvh=1, d=128,
                    prefix=[70, 99, 0]),

@@ -109,6 +109,18 @@ def test_decode_refuses(change, words):
         ops.paged_decode_op(*args, **change.get("kw", {}))
 
 
+@pytest.mark.parametrize("kw, words", [
+    (dict(softcap=-1.0), "softcap"), (dict(softcap=1e-7), "softcap"),
+    (dict(softcap=1e4), "softcap"), (dict(softcap=float("nan")), "softcap"),
+    (dict(scale=1e31), "scale"), (dict(scale=-float("inf")), "scale"),
+    (dict(scale=float("nan")), "scale")])
+def test_scores_refuse(kw, words):
+    with pytest.raises(ValueError, match=words):
+        ops.paged_decode_op(*_decode_args()[0], **kw)
+    with pytest.raises(ValueError, match=words):
+        ops.flash_prefill_packed_op(*_packed_args(), **kw)
+
+
 def test_decode_refuses_overlap_and_gradients():
     args, room = _decode_args()
     store = torch.zeros(2 * 2 * room + 8)

@@ -16,7 +16,6 @@ allocate what they need from torch's allocator, and offer no gradients.
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -158,10 +157,12 @@ def _score_args(scale, softcap, slopes, d, qh, kvh, dev):
         _refuse(f"q: {qh} heads are no multiple of the {kvh} key heads")
     scale = d ** -0.5 if scale is None else float(scale)
     softcap = float(softcap)
-    if not math.isfinite(scale):
-        _refuse(f"scale: finite, got {scale}")
-    if not 0.0 <= softcap < math.inf:
-        _refuse(f"softcap: finite and not negative, got {softcap}")
+    if not -1e30 <= scale <= 1e30:  # and its quotient by a cap in 32 bits
+        _refuse(f"scale: from -1e30 to 1e30, got {scale}")
+    # The kernels take the tanh from one exponential, whose error is the
+    # cap's size times 2^-23: 3e-4 of a logit at the largest.
+    if softcap and not 1e-6 <= softcap <= 1000.0:
+        _refuse(f"softcap: 0 or from 1e-6 to 1000, got {softcap}")
     if slopes is not None:
         _array("slopes", slopes, _F32, (qh,), dev)
     return scale, softcap
@@ -258,11 +259,11 @@ def paged_decode_op(q: torch.Tensor, k_pool: torch.Tensor,
     append first). d is 64 or 128; qh is a multiple of kvh.
 
     A score is s = scale * q.k (scale: d ** -0.5 by default), then
-    softcap * tanh(s / softcap) if softcap > 0, then less slopes[h] * |i-j|
-    if `slopes` [qh] fp32 are given, with the query's position i and the
-    key's position j: the last slot's and the key's slot number, or
-    `q_pos` [B] and `key_pos` [B, kvh, room] int32 for a cache whose rows
-    have moved.
+    softcap * tanh(s / softcap) for a softcap from 1e-6 to 1000 (0: none),
+    then less slopes[h] * |i-j| if `slopes` [qh] fp32 are given, with the
+    query's position i and the key's position j: the last slot's and the
+    key's slot number, or `q_pos` [B] and `key_pos` [B, kvh, room] int32 for
+    a cache whose rows have moved.
 
     `mass` [B, kvh, room] fp32 asks for the attention weights: returned is
     mass plus, for each slot, the weights that the key head's query heads
