@@ -133,6 +133,10 @@ def test_decode_refuses_overlap_and_gradients():
         ops.paged_decode_op(*args)
     with torch.no_grad():
         ops.paged_decode_op(*args)
+    args[0].requires_grad_(False)
+    args[2] = args[2].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.paged_decode_op(*args)
 
 
 def _packed_args():
@@ -166,6 +170,20 @@ def test_packed_refuses_overlap_and_keeps_rows():
     q, k, v, cu = _packed_args()
     with pytest.raises(ValueError, match="apart"):
         ops.flash_prefill_packed_op(q, k, v, cu, out=q)
+    row = torch.zeros(64 * 40).bfloat16()
+    for strides in ((256, 0, 1), (0, 64, 1), (64, 64, 1), (256, 56, 1),
+                    (200, 64, 1)):
+        with pytest.raises(ValueError, match="share"):
+            ops.flash_prefill_packed_op(
+                q, k, v, cu, out=row.as_strided((9, 4, 64), strides))
+    for strides in ((256, 64, 1), (64, 9 * 64, 1), (264, 64, 1)):
+        ops.flash_prefill_packed_op(
+            q, k, v, cu, out=row.as_strided((9, 4, 64), strides))
+    for one in (q[:1], q[:, :1]):  # a stride that nothing steps by
+        args = [one, k[:len(one), :1], v[:len(one), :1], cu[:1].repeat(2)]
+        ops.flash_prefill_packed_op(
+            *args, out=row.as_strided(one.shape, (
+                (0, 64, 1) if len(one) == 1 else (64, 0, 1))))
     out = torch.full_like(q, 7.0)
     ops.flash_prefill_packed_op(q, k, v, cu[:2], out=out)
     assert (out[4:] == 7).all() and not (out[:4] == 7).any()

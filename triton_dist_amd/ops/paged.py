@@ -114,6 +114,9 @@ def _cache(k_pool, v_pool, block_table, seq_lens):
         _refuse(f"k_pool: bfloat16 or float16, got {dtype}")
     if v_pool.dtype != dtype or v_pool.shape != shape or v_pool.device != dev:
         _refuse("v_pool: of k_pool's type, shape and device")
+    if (k_pool.requires_grad or v_pool.requires_grad) \
+            and torch.is_grad_enabled():
+        _no_backward()
     n, block, kvh, d = shape
     if not (0 < n < 1 << 31 and block > 0 and kvh > 0 and d > 0) or d & 7:
         _refuse("k_pool: from 1 to 2^31 - 1 pages of at least one slot and "
@@ -524,6 +527,12 @@ def flash_prefill_packed_op(q: torch.Tensor, k: torch.Tensor,
         if out.shape != q.shape:
             _refuse(f"out: of q's shape, got {tuple(out.shape)}")
         _heads("out", out, dtype, dev)
+        (x, n), (y, more) = sorted(zip(out.stride(), out.shape[:2]))
+        if n > 1 and x < d or more > 1 and y < (x * (n - 1) if n > 1
+                                                else 0) + d:
+            _refuse("out: rows that do not share memory")
+        if out.requires_grad and torch.is_grad_enabled():
+            _no_backward()
         if _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
             _refuse("out: apart from q, k and v")
     lse = torch.empty((rows, qh), dtype=_F32, device=dev) \
