@@ -1,0 +1,129 @@
+"""Inputs at the ends of what the operators over a paged cache and packed
+prompts take, and what a right answer is there."""
+import torch
+
+import paged_oracle as oracle
+
+F32 = oracle.F32
+
+
+def whole(gen, shape, dtype, size=1.0):
+    """Whole numbers from -4 to 4, times a power of two: their products add
+    up without a rounding in 32 bits."""
+    return (torch.randint(-4, 5, shape, generator=gen) * size).to(dtype)
+
+
+def seen_by(m, n, causal, prefix):
+    at, j = torch.arange(m)[:, None] + n - m, torch.arange(n)
+    if not causal:
+        return at, j, torch.ones(m, n, dtype=torch.bool)
+    return at, j, (j <= at) | (j < prefix)
+
+
+def pick(s, off, seen, v, dtype):
+    """Scores s [m, n] in 64 bits, which 32 bits hold to `off`, over values
+    v [n, d]: the least and largest output that scores so far off can give.
+    Other keys than those within 60 of the top weigh e^-60 at most. Where
+    `off` is 0 the keys at the top share it evenly, if no other is near."""
+    s = torch.where(seen, s, float("-inf"))
+    top, at = s.max(1, keepdim=True)
+    slack = off + off.gather(1, at)
+    near = seen & (s >= top - slack - 60)
+    even = ((s == top) == near).all() and not off.any()
+    low = torch.empty(len(s), v.shape[1], dtype=torch.float64)
+    high = low.clone()
+    for r in range(len(s)):
+        x = v[near[r]]
+        if even:
+            low[r] = high[r] = x.mean(0)
+        else:
+            low[r], high[r] = x.min(0).values, x.max(0).values
+        # a weight and the output are rounded once each
+        tol = (2 * oracle.HALF_STEP[dtype] + 2 * len(s[0]) * F32) \
+            * x.abs().mean(0) if even else \
+            2 * oracle.HALF_STEP[dtype] * x.abs().max(0).values
+        low[r] -= tol + 1e-12
+        high[r] += tol + 1e-12
+    return low, high, torch.logsumexp(s, 1), slack[:, 0]
+
+
+# name: type, d, scale, size of q and k, slope, cap, causal
+LARGE = {
+    "below": (torch.bfloat16, 64, 3e3, 1, 0.0, 0.0, True),
+    "about": (torch.float16, 128, -2e4, 1, 0.0, 0.0, True),
+    "million": (torch.bfloat16, 128, 1e6, 1, 0.0, 0.0, False),
+    "1e8": (torch.bfloat16, 64, 1e8, 1, 0.0, 0.0, True),
+    "-1e10": (torch.bfloat16, 128, -1e10, 1, 0.0, 0.0, True),
+    "1e30": (torch.float16, 128, 1e30, 1, 0.0, 0.0, True),
+    "1e30_64": (torch.float16, 64, 1e30, 1, 0.0, 0.0, False),
+    "inputs": (torch.bfloat16, 128, 1.0, 2.0 ** 40, 0.0, 0.0, True),
+    "inputs_16": (torch.float16, 64, 1.0, 1024, 0.0, 0.0, True),
+    "both": (torch.bfloat16, 64, 1e8, 1, 1e8, 0.0, True),
+    "both_16": (torch.float16, 128, 1e10, 1, 3e9, 0.0, True),
+    "slope": (torch.bfloat16, 128, 1.0, 1, 1e9, 0.0, False),
+    "slope_16": (torch.float16, 64, 0.5, 1, 1e12, 0.0, True),
+    "capped": (torch.bfloat16, 64, 1.0, 1, 1e9, 30.0, True),
+    "capped_16": (torch.float16, 128, 1.0, 1, 1e7, 50.0, False),
+    "flat": (torch.bfloat16, 128, 1e9, 1, 1.0, 0.0, True),
+    "cap_alone": (torch.bfloat16, 64, 1e9, 1, 0.0, 1000.0, True),
+}
+
+
+def scores(q, k, scale, cap, bias):
+    """In 64 bits, and how far 32 bits may be off: whole numbers' products
+    are exact, and a scale alone keeps their order and what is equal."""
+    s = (q.double() @ k.double().t()) * scale
+    off = torch.zeros_like(s)
+    if cap:
+        s = cap * torch.tanh(s / cap)
+        off += 8 * F32 * cap
+    if bias is not None:
+        off += 16 * F32 * (s.abs() + bias.abs())
+        s = s - bias
+    return s, off
+
+
+def packed_large(name):
+    """Two documents; returns the call's arguments and what to hold the
+    outputs against."""
+    dtype, d, scale, size, slope, cap, causal = LARGE[name]
+    gen = torch.Generator().manual_seed(len(name))
+    lens, qh, kvh = [300, 65], 4, 2
+    rows = sum(lens)
+    q = whole(gen, (rows, qh, d), dtype, size)
+    k = whole(gen, (rows, kvh, d), dtype, size)
+    v = torch.randn(rows, kvh, d, generator=gen).to(dtype)
+    prefix = torch.tensor([0, 40], dtype=torch.int32)
+    cu = torch.tensor([0, 300, 365], dtype=torch.int32)
+    kw = dict(scale=scale, softcap=cap, causal=causal, prefix_lens=prefix)
+    if slope:
+        kw["slopes"] = slope * 2.0 ** -torch.arange(qh)
+    want = {x: torch.zeros(rows, qh, d, dtype=torch.float64)
+            for x in ("low", "high")}
+    want["lse"] = torch.zeros(rows, qh, dtype=torch.float64)
+    want["off"] = torch.zeros_like(want["lse"])
+    for i, n in enumerate(lens):
+        a, e = int(cu[i]), int(cu[i + 1])
+        at, j, seen = seen_by(n, n, causal, int(prefix[i]))
+        for h in range(qh):
+            bias = float(kw["slopes"][h]) * (at - j).abs().double() \
+                if slope else None
+            s, off = scores(q[a:e, h], k[a:e, h * kvh // qh], scale, cap,
+                            bias)
+            low, high, lse, slack = pick(
+                s, off, seen, v[a:e, h * kvh // qh].double(), dtype)
+            want["low"][a:e, h], want["high"][a:e, h] = low, high
+            want["lse"][a:e, h], want["off"][a:e, h] = lse, slack
+    return (q, k, v, cu), kw, want
+
+
+def hold(out, lse, want):
+    out, lse = out.detach().cpu().double(), lse.detach().cpu().double()
+    ok = (out >= want["low"]) & (out <= want["high"])
+    bad = (~ok).nonzero()
+    assert not len(bad), (
+        f"{len(bad)} of {ok.numel()}, first at {bad[0].tolist()}: "
+        f"{float(out[~ok][0])}, not from {float(want['low'][~ok][0])} to "
+        f"{float(want['high'][~ok][0])}")
+    tol = 8 * F32 * want["lse"].abs() + want["off"] + 1e-5
+    assert ((lse - want["lse"]).abs() <= tol).all()
