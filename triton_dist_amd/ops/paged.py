@@ -329,10 +329,15 @@ def paged_decode_op(q: torch.Tensor, k_pool: torch.Tensor,
 
 def _weights_cpu(s: torch.Tensor):
     """Softmax over the last axis and its log-sum-exp; rows of -inf weigh
-    nothing."""
-    lse = torch.logsumexp(s, -1)
-    w = torch.exp(s - torch.where(torch.isinf(lse), 0.0, lse)[..., None])
-    return torch.where(torch.isinf(s) & (s < 0), 0.0, w), lse
+    nothing. The maximum and the sum stay apart, since a large maximum
+    swallows the log of the sum."""
+    if not s.shape[-1]:
+        return s, s.new_full(s.shape[:-1], float("-inf"))
+    top = s.amax(-1, keepdim=True)
+    e = torch.exp(s - torch.where(top == float("-inf"), 0.0, top))
+    total = e.sum(-1, keepdim=True)
+    w = e / torch.where(total == 0, 1.0, total)
+    return w, (top + torch.log(total))[..., 0]
 
 
 def _decode_cpu(q, k_pool, v_pool, table, lens, scale, softcap, slopes,
