@@ -19,3 +19,15 @@ def test_packed_large_logits(name):
           for k, x in kw.items()}
     out, lse = ops.flash_prefill_packed_op(*args, return_lse=True, **kw)
     limits.hold(out, lse, want)
+
+
+@pytest.mark.parametrize("name", limits.LARGE)
+def test_decode_large_logits(name):
+    """The same, with equal keys in chunks apart, and their weights."""
+    args, kw, want = limits.decode_large(name)
+    args = [x.cuda() for x in args]
+    kw = {k: x.cuda() if isinstance(x, torch.Tensor) else x
+          for k, x in kw.items()}
+    out, lse, mass = ops.paged_decode_op(*args, return_lse=True, **kw)
+    limits.hold(out, lse, want)
+    limits.hold_mass(mass, want)

@@ -112,6 +112,17 @@ TD_DEV void wave_fence() {
   asm volatile("" ::: "memory");
 }
 
+// The power of two of a rounded logit less a maximum of such: taken off the
+// unrounded product, the largest would differ by its maximum's rounding.
+TD_DEV float power_of(float logit, float top) {
+#pragma clang fp contract(off)
+  return __builtin_amdgcn_exp2f(logit - top);
+}
+
+TD_DEV float lse_of(float top, float sum) {
+  return sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
 struct Chunk {
   int b, len;        // sequence and its length
   int first, count;  // this chunk's number among the sequence's, how many
@@ -120,7 +131,10 @@ struct Chunk {
 // Where a call keeps what its kernels hand on.
 struct DecodeWork {
   float *part;    // [chunks, qh, d]: outputs of one chunk among several
-  float *sum;     // [chunks, qh]: log2 of a chunk's sum
+  // [chunks, qh]: a chunk's largest logit, in units of log2, and the sum of
+  // its powers less that one. They stay apart, since past 2^24 a maximum
+  // swallows the log of its sum.
+  float2 *sum;
   int *plan;      // [batch, 2]: a sequence's chunks, its first further one
   float *logits;  // [batch, qh, room], in units of log2, where weights are
   int groups;     // of up to 16 query heads of a key head
@@ -418,7 +432,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(s[t][i] - safe);
+        const float p = power_of(s[t][i], safe);
         l += p;
         hi[4 * t + i] = (T)p;
         lo[4 * t + i] = (T)(p - (float)hi[4 * t + i]);
@@ -440,7 +454,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
   if (!cut.shared) {
     if (n >= heads) return;
     const float r = l == 0.f ? 0.f : 1.f / l;
-    const float lse = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
     const long at = (long)id * a.qh + h0 + n, to = (long)b * a.qh + h0 + n;
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
@@ -455,8 +468,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
       }
     }
     if (qd == 0) {
-      w.sum[at] = lse;
-      if (ch.count == 1 && a.lse) a.lse[to] = lse * kLn2;
+      w.sum[at] = make_float2(m, l);
+      if (ch.count == 1 && a.lse) a.lse[to] = lse_of(m, l);
     }
     return;
   }
@@ -484,17 +497,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
       o += r * *(const f32x4 *)((const float *)lds[x] + h * kORow + c);
     }
     o *= sum == 0.f ? 0.f : 1.f / sum;
-    const float lse = sum == 0.f ? -INFINITY
-                                 : top + __builtin_amdgcn_logf(sum);
     const long at = (long)id * a.qh + h0 + h, to = (long)b * a.qh + h0 + h;
     if (ch.count == 1) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) ((T *)a.out)[to * D + c + x] = (T)o[x];
-      if (c == 0 && a.lse) a.lse[to] = lse * kLn2;
+      if (c == 0 && a.lse) a.lse[to] = lse_of(top, sum);
     } else {
       *(f32x4 *)(w.part + at * D + c) = o;
     }
-    if (c == 0) w.sum[at] = lse;
+    if (c == 0) w.sum[at] = make_float2(top, sum);
   }
 }
 
@@ -507,7 +518,8 @@ constexpr int kSpanWaves = 8;
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kSpanWaves) void k_decode_finish(PagedDecodeArgs a,
                                                          DecodeWork w) {
-  __shared__ float lds_lse[kSpanWaves], lds_o[kSpanWaves][D];
+  __shared__ float lds_top[kSpanWaves], lds_sum[kSpanWaves];
+  __shared__ float lds_o[kSpanWaves][D];
   const int b = blockIdx.x, kh = blockIdx.y, z = blockIdx.z;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int g = a.qh / a.c.kvh, room = a.c.room();
@@ -515,17 +527,18 @@ __global__ __launch_bounds__(64 * kSpanWaves) void k_decode_finish(PagedDecodeAr
   auto row = [&](int i, int h) {  // a chunk's outputs of a query head
     return (long)(i ? more + i - 1 : b) * a.qh + h;
   };
-  auto lse_of = [&](int h) {  // the whole wave
-    float top = -INFINITY;
+  // all chunks' maximum and the sum of powers less that, by the whole wave
+  auto sum_of = [&](int h, float &top, float &sum) {
+    top = -INFINITY, sum = 0.f;
     for (int i = lane; i < count; i += 64)
-      top = fmaxf(top, w.sum[row(i, h)]);
+      top = fmaxf(top, w.sum[row(i, h)].x);
     top = wave_max(top);
-    const float safe = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int i = lane; i < count; i += 64)
-      sum += __builtin_amdgcn_exp2f(w.sum[row(i, h)] - safe);
+    if (top == -INFINITY) top = 0.f;  // nothing to sum
+    for (int i = lane; i < count; i += 64) {
+      const float2 x = w.sum[row(i, h)];
+      sum += __builtin_amdgcn_exp2f(x.x - top) * x.y;
+    }
     sum = wave_sum(sum);
-    return sum == 0.f ? -INFINITY : safe + __builtin_amdgcn_logf(sum);
   };
   if (z < w.joins) {
     if (count == 1) return;
@@ -537,13 +550,15 @@ __global__ __launch_bounds__(64 * kSpanWaves) void k_decode_finish(PagedDecodeAr
       const bool live = wave < each * at_once && y < heads &&
                         z * heads + y < g;
       if (live) {
-        const float lse = lse_of(h);
-        const float safe = lse == -INFINITY ? 0.f : lse;
+        float top, sum;
+        sum_of(h, top, sum);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         float o[D / 64] = {};
 #pragma unroll 4
         for (int i = wave % each; i < count; i += each) {
           const long at = row(i, h);
-          const float r = __builtin_amdgcn_exp2f(w.sum[at] - safe);
+          const float2 x = w.sum[at];
+          const float r = __builtin_amdgcn_exp2f(x.x - top) * x.y * inv;
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
             o[c] += r * w.part[at * D + lane * (D / 64) + c];
@@ -552,7 +567,7 @@ __global__ __launch_bounds__(64 * kSpanWaves) void k_decode_finish(PagedDecodeAr
         for (int c = 0; c < D / 64; ++c)
           lds_o[wave][lane * (D / 64) + c] = o[c];
         if (wave % each == 0 && lane == 0 && a.lse)
-          a.lse[(long)b * a.qh + h] = lse * kLn2;
+          a.lse[(long)b * a.qh + h] = lse_of(top, sum);
       }
       __syncthreads();
       for (int i = tid; i < at_once * D; i += 64 * kSpanWaves) {
@@ -584,17 +599,19 @@ __global__ __launch_bounds__(64 * kSpanWaves) void k_decode_finish(PagedDecodeAr
                             ? s[(long)y * room + i * 64 * kSpanWaves]
                             : -INFINITY;
         }
-      const float lse = x + wave < g ? lse_of(kh * g + x + wave) : -INFINITY;
+      float top = 0.f, total = 0.f;
+      if (x + wave < g) sum_of(kh * g + x + wave, top, total);
       __syncthreads();
-      if (lane == 0) lds_lse[wave] = lse;
+      if (lane == 0) lds_top[wave] = top, lds_sum[wave] = total;
       __syncthreads();
 #pragma unroll
       for (int y = 0; y < kSpanWaves; ++y) {
-        const float total = lds_lse[y];
-        if (total == -INFINITY) continue;  // also a head that is not there
+        const float most = lds_top[y], all = lds_sum[y];
+        if (all == 0.f) continue;  // also a head that is not there
+        const float inv = 1.f / all;
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
-          sum[i] += __builtin_amdgcn_exp2f(logit[y][i] - total);
+          sum[i] += __builtin_amdgcn_exp2f(logit[y][i] - most) * inv;
       }
     }
 #pragma unroll
@@ -917,7 +934,7 @@ static long decode_chunks(int batch, int kvh, const DecodeWork &w) {
 size_t paged_decode_workspace(int batch, int qh, int kvh, int d, long room,
                               bool mass) {
   const size_t chunks = decode_chunks(batch, kvh, decode_work(batch, qh, kvh));
-  return (chunks * qh * (d + 1) + 2 * (size_t)batch +
+  return (chunks * qh * (d + 2) + 2 * (size_t)batch +
           (mass ? (size_t)batch * qh * room : 0)) *
          sizeof(float);
 }
@@ -952,7 +969,7 @@ void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
   DecodeWork w = decode_work(a.c.batch, a.qh, a.c.kvh);
   w.part = (float *)a.ws;
   const size_t chunks = decode_chunks(a.c.batch, a.c.kvh, w);
-  w.sum = w.part + chunks * a.qh * a.c.d;
+  w.sum = (float2 *)(w.part + chunks * a.qh * a.c.d);
   w.plan = (int *)(w.sum + chunks * a.qh);
   w.logits = a.mass ? (float *)(w.plan + 2 * (size_t)a.c.batch) : nullptr;
   if (a.c.is_fp16)
