@@ -2,6 +2,7 @@
 prompts take, and what a right answer is there."""
 import torch
 
+import paged_cases as cases
 import paged_oracle as oracle
 
 F32 = oracle.F32
@@ -194,3 +195,82 @@ def hold_mass(mass, want):
         # equal keys share evenly, others get nothing: a few roundings
         assert ((mass - want["mass"]).abs()
                 <= 64 * F32 * (1 + want["mass"])).all()
+
+
+def plant(rows):
+    """Infinities and NaN into rows [n, ...] of values that are seen."""
+    n = len(rows)
+    rows[n - 1, ..., ::7] = float("inf")
+    rows[n // 2, ..., 5::16] = float("nan")
+    rows[0, ..., 3::11] = -float("inf")
+
+
+def wild_sums(v, seen):
+    """What values v [n, d] that are not finite make of outputs whose keys
+    are `seen` [m, n], whatever the weights; 0 where there are none."""
+    wild = torch.where(torch.isfinite(v), 0.0, v.double())
+    total = torch.zeros(len(seen), v.shape[1], dtype=torch.float64)
+    for j in wild.ne(0).any(1).nonzero()[:, 0].tolist():
+        total[seen[:, j]] += wild[j]
+    return total
+
+
+# cases of decode whose chunks are cut alike and unlike, and one whose
+# weights mostly underflow
+DECODE_WILD = ["odd", "ten_to_one", "sixteen", "fp16", "long", "sloped",
+               "moved", "mass", "missing", "head_major", "strong",
+               "bigger_mass", "bigger_groups", "big_ragged"]
+
+
+def decode_wild(name):
+    q, st, kw = cases.decode_inputs(name)
+    k, v, table, lens = st["k"], st["v"], st["table"], st["lens"]
+    n_blocks, block, kvh, d = v.shape
+    calm = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    for b in range(len(lens)):  # the oracle has its rows without them
+        slots = torch.arange(int(lens[b]))
+        page = table[b].long()[slots // block]
+        there = (page >= 0) & (page < n_blocks)
+        if there.any():
+            at = page[there], slots[there] % block
+            rows = v[at].clone()
+            plant(rows)
+            v[at] = rows
+    want = oracle.decode(q, k, calm, table, lens, **kw)
+    out = want["out"][0]
+    for b in range(len(lens)):
+        for h in range(q.shape[1]):
+            rows, _ = oracle.gather(v, table[b], range(int(lens[b])),
+                                    h * kvh // q.shape[1])
+            more = wild_sums(rows, torch.ones(1, len(rows)).bool())[0]
+            out[b, h] = torch.where(more == 0, out[b, h], more)
+    return q, st, kw, want
+
+
+PACKED_WILD = ["odd", "ten_to_one", "fp16", "long", "full", "capped",
+               "prefix", "all", "more_keys", "fewer_keys", "tail", "strong",
+               "steep", "rising", "wild_16", "many_128"]
+
+
+def packed_wild(name):
+    q, k, v, cu, kw = cases.packed_inputs(name)
+    kcu = kw.get("cu_seqlens_k", cu)
+    docs = range(len(cu) - 1)
+    calm = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    for i in docs:
+        a, e = int(kcu[i]), int(kcu[i + 1])
+        if a < e:
+            plant(v[a:e])
+    want = cases.packed_expected(q, k, calm, cu, kw)
+    out = want["out"][0]
+    for i in docs:
+        q0, q1, k0, k1 = (int(x) for x in (cu[i], cu[i + 1], kcu[i],
+                                           kcu[i + 1]))
+        p = int(kw["prefix_lens"][i]) if "prefix_lens" in kw else 0
+        _, _, seen = seen_by(q1 - q0, k1 - k0, kw["causal"], p)
+        for h in range(q.shape[1]):
+            more = wild_sums(v[k0:k1, h * k.shape[1] // q.shape[1]], seen)
+            # where a score is none, nothing else counts
+            out[q0:q1, h] = torch.where((more == 0) | out[q0:q1, h].isnan(),
+                                        out[q0:q1, h], more)
+    return (q, k, v, cu), kw, want

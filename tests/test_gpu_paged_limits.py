@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import paged_limits as limits
+import paged_oracle as oracle
 from triton_dist_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -31,3 +32,18 @@ def test_decode_large_logits(name):
     out, lse, mass = ops.paged_decode_op(*args, return_lse=True, **kw)
     limits.hold(out, lse, want)
     limits.hold_mass(mass, want)
+
+
+def _cuda(x):
+    return {k: _cuda(v) for k, v in x.items()} if isinstance(x, dict) else \
+        x.cuda() if isinstance(x, torch.Tensor) else x
+
+
+@pytest.mark.parametrize("name", limits.DECODE_WILD)
+def test_decode_wild_values(name):
+    """Values that are no finite numbers, among slots that are seen."""
+    q, st, kw, want = limits.decode_wild(name)
+    g = _cuda(st)
+    out = ops.paged_decode_op(q.cuda(), g["k"], g["v"], g["table"],
+                              g["lens"], **_cuda(kw))
+    oracle.check("out", out[0] if "mass" in kw else out, want["out"])

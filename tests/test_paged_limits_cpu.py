@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import paged_limits as limits
+import paged_oracle as oracle
 from triton_dist_amd import ops
 
 
@@ -20,3 +21,18 @@ def test_decode_large_logits(name):
     out, lse, mass = ops.paged_decode_op(*args, return_lse=True, **kw)
     limits.hold(out, lse, want)
     limits.hold_mass(mass, want)
+
+
+@pytest.mark.parametrize("name", limits.DECODE_WILD)
+def test_decode_wild_values(name):
+    q, st, kw, want = limits.decode_wild(name)
+    out = ops.paged_decode_op(q, st["k"], st["v"], st["table"], st["lens"],
+                              **kw)
+    oracle.check("out", out[0] if "mass" in kw else out, want["out"])
+
+
+@pytest.mark.parametrize("name", limits.PACKED_WILD)
+def test_packed_wild_values(name):
+    args, kw, want = limits.packed_wild(name)
+    oracle.check("out", ops.flash_prefill_packed_op(*args, **kw),
+                 want["out"])

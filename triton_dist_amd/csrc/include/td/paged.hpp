@@ -89,6 +89,14 @@ TD_DEV int wave_scan(int x) {
   return x;
 }
 
+// Infinite or not a number.
+TD_DEV bool wild(__bf16 x) {
+  return (__builtin_bit_cast(unsigned short, x) & 0x7f80) == 0x7f80;
+}
+TD_DEV bool wild(_Float16 x) {
+  return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
+}
+
 // How a score becomes a logit: capped by a tanh, then lowered by the
 // distance between the query's and the key's position.
 struct ScoreArgs {

@@ -123,6 +123,12 @@ TD_DEV float lse_of(float top, float sum) {
   return sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
+// A part's share in a sum. One that is no finite number counts in full,
+// however small its share is.
+TD_DEV float share_of(float r, float x) {
+  return fabsf(x) < INFINITY ? r * x : x;
+}
+
 struct Chunk {
   int b, len;        // sequence and its length
   int first, count;  // this chunk's number among the sequence's, how many
@@ -451,6 +457,40 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
 
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
+  // A value that is no finite number makes its outputs so, however small its
+  // weight. Times a weight that underflows, or a rounded weight's rest of
+  // zero or less, an infinite one is NaN, so outputs that are NaN without a
+  // score being one are summed again from such values alone.
+  bool spoilt = false;
+#pragma unroll
+  for (int t = 0; t < kT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) spoilt |= acc[t][i] != acc[t][i];
+  if (__any(spoilt && l == l)) {
+    f32x4 alone[kT] = {};
+    for (base = k0 + (cut.shared ? wave * kTile : 0); base < k1;
+         base += stride)
+      for (int slot = base; slot < min(base + kTile, k1); ++slot) {
+        const long p = a.c.page(b, slot);
+        if (p < 0) continue;
+        const T *row = (const T *)a.c.v + kh * a.c.v_head + p * a.c.v_page +
+                       (long)((unsigned)slot % (unsigned)a.c.block) *
+                           a.c.v_row + qd * 4;
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          const vec4<T> x = *(const vec4<T> *)(row + t * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            alone[t][i] += wild(x[i]) ? (float)x[i] : 0.f;
+        }
+      }
+#pragma unroll
+    for (int t = 0; t < kT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (acc[t][i] != acc[t][i] && alone[t][i] != 0.f)
+          acc[t][i] = alone[t][i];
+  }
   if (!cut.shared) {
     if (n >= heads) return;
     const float r = l == 0.f ? 0.f : 1.f / l;
@@ -494,7 +534,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
     for (int x = 0; x < 4; ++x) {
       const float r = __builtin_amdgcn_exp2f(lds_m[x][h] - safe);
       sum += r * lds_l[x][h];
-      o += r * *(const f32x4 *)((const float *)lds[x] + h * kORow + c);
+      const f32x4 y = *(const f32x4 *)((const float *)lds[x] + h * kORow + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += share_of(r, y[e]);
     }
     o *= sum == 0.f ? 0.f : 1.f / sum;
     const long at = (long)id * a.qh + h0 + h, to = (long)b * a.qh + h0 + h;
@@ -561,7 +603,7 @@ __global__ __launch_bounds__(64 * kSpanWaves) void k_decode_finish(PagedDecodeAr
           const float r = __builtin_amdgcn_exp2f(x.x - top) * x.y * inv;
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
-            o[c] += r * w.part[at * D + lane * (D / 64) + c];
+            o[c] += share_of(r, w.part[at * D + lane * (D / 64) + c]);
         }
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)

@@ -275,7 +275,8 @@ def paged_decode_op(q: torch.Tensor, k_pool: torch.Tensor,
 
     Returns out [B, qh, d], and in this order, where asked for, the log of
     the sum of exponentials [B, qh] fp32 and the weights. A sequence that
-    sees no key gets zeros and -inf.
+    sees no key gets zeros and -inf. A value that is no finite number counts
+    in full, however small its weight is.
     """
     fields, (block, kvh, d, b, room) = _cache(k_pool, v_pool, block_table,
                                               seq_lens)
@@ -340,6 +341,19 @@ def _weights_cpu(s: torch.Tensor):
     return w, (top + torch.log(total))[..., 0]
 
 
+def _sums_cpu(w, v, seen):
+    """w [..., m, n] times v [..., n, d]; a value that is no finite number
+    counts for the rows that see it, `seen` [m, n], however small its weight
+    is, and for no other."""
+    wild = ~torch.isfinite(v)
+    o = torch.matmul(w, torch.where(wild, 0.0, v))
+    keys = wild.any(-1).flatten(0, -2).any(0).nonzero()[:, 0]
+    for j in keys.tolist():
+        o[..., seen[:, j], :] += torch.where(
+            wild[..., j, None, :], v[..., j, None, :], 0.0)
+    return o
+
+
 def _decode_cpu(q, k_pool, v_pool, table, lens, scale, softcap, slopes,
                 key_pos, q_pos, mass, mass_out, out, lse):
     n_blocks, block, kvh, d = k_pool.shape
@@ -360,7 +374,8 @@ def _decode_cpu(q, k_pool, v_pool, table, lens, scale, softcap, slopes,
                 gap = gap[there].expand(kvh, -1)
             s = s - slopes.view(kvh, g, 1) * gap.abs().float()[:, None]
         w, total = _weights_cpu(s)
-        out[b] = torch.matmul(w, v).view(-1, d).to(out.dtype)
+        out[b] = _sums_cpu(w, v, torch.ones(g, len(at), dtype=torch.bool)) \
+            .view(-1, d).to(out.dtype)
         lse[b] = total.view(-1)
         if mass is not None:
             new = mass[b].clone()
@@ -488,7 +503,9 @@ def flash_prefill_packed_op(q: torch.Tensor, k: torch.Tensor,
     exponentials [T, qh] fp32. A row that sees no key gets zeros and -inf.
     Rows that belong to no document are left as they were in a given `out`,
     and are zeros and -inf in tensors that the call makes (a `lse` always).
-    What the mask hides from a query does not count, whatever it holds.
+    What the mask hides from a query does not count, whatever it holds; a
+    value that is seen and is no finite number counts in full, however small
+    its weight is.
     """
     dev, dtype = q.device, q.dtype
     if q.dim() != 3 or k.dim() != 3:
@@ -589,11 +606,7 @@ def _packed_cpu(q, k, v, cu_q, cu_k, causal, prefix, scale, softcap, slopes,
             s = s.masked_fill(~seen, float("-inf"))
         w, total = _weights_cpu(s)
         vf = v[k0:k0 + n].float().transpose(0, 1)   # [kvh, n, d]
-        wild = ~torch.isfinite(vf)
-        o = torch.matmul(w, torch.where(wild, 0.0, vf)[:, None])
-        for key in wild.any(-1).any(0).nonzero()[:, 0].tolist():
-            o[:, :, seen[:, key]] += torch.where(
-                wild[:, key], vf[:, key], 0.0)[:, None, None]
+        o = _sums_cpu(w, vf[:, None], seen)
         out[q0:q1] = o.permute(2, 0, 1, 3).reshape(m, qh, d).to(out.dtype)
         if lse is not None:
             lse[q0:q1] = total.permute(2, 0, 1).reshape(m, qh)
