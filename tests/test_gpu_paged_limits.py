@@ -47,3 +47,10 @@ def test_decode_wild_values(name):
     out = ops.paged_decode_op(q.cuda(), g["k"], g["v"], g["table"],
                               g["lens"], **_cuda(kw))
     oracle.check("out", out[0] if "mass" in kw else out, want["out"])
+
+
+@pytest.mark.parametrize("name", limits.PACKED_WILD)
+def test_packed_wild_values(name):
+    args, kw, want = limits.packed_wild(name)
+    out = ops.flash_prefill_packed_op(*(x.cuda() for x in args), **_cuda(kw))
+    oracle.check("out", out, want["out"])

@@ -73,14 +73,6 @@ TD_DEV s16x4 read_transposed(const void *lds) {
 template <int D> constexpr int kRowK = D + 8;
 template <int D> constexpr int kRowV = D + 32;
 
-// Infinite or not a number.
-TD_DEV bool wild(bf16 x) {
-  return (__builtin_bit_cast(unsigned short, x) & 0x7f80) == 0x7f80;
-}
-TD_DEV bool wild(_Float16 x) {
-  return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
-}
-
 struct Doc {
   int q0, k0;  // first row, first key
   int m, n;    // rows, keys
@@ -509,6 +501,33 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 2) void k_packed_prefill(
         }
     }
   l += __shfl_xor(l, 32);
+  // A value that is no finite number makes its outputs so, however small its
+  // weight; times one that underflows an infinite value is NaN. So outputs
+  // that are NaN without a score being one are summed from such values alone.
+  bool spoilt = false;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) spoilt |= acc[t][r] != acc[t][r];
+  if (__any(spoilt && l == l)) {
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      f32x16 alone = {};
+      for (int key = 0; key < most; ++key) {
+        if (key >= lim) continue;
+        const T *v = (const T *)a.v + (long)(doc.k0 + key) * a.v_tok +
+                     kh * a.v_head + 4 * h + 32 * t;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const T x = v[8 * (r / 4) + r % 4];
+          alone[r] += wild(x) ? (float)x : 0.f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (acc[t][r] != acc[t][r] && alone[r] != 0.f) acc[t][r] = alone[r];
+    }
+  }
   if (!live) return;
   if (a.lse && h == 0 && row0 + c < doc.m)
     a.lse[(long)(doc.q0 + row) * a.qh + head] =
