@@ -274,3 +274,42 @@ def packed_wild(name):
             out[q0:q1, h] = torch.where((more == 0) | out[q0:q1, h].isnan(),
                                         out[q0:q1, h], more)
     return (q, k, v, cu), kw, want
+
+
+# many keys of a small weight beside a few of a large one that hold zeros:
+# d, keys, steps of 2 of the small weight, and how the large ones come
+FAINT = {
+    "first": (64, 700, 25.5, "first"), "last": (128, 700, 25.5, "last"),
+    "rising": (64, 900, 22.0, "rising"), "fainter": (128, 3000, 28.0,
+                                                     "first"),
+    "mild": (64, 500, 15.5, "last"),
+}
+
+
+def faint(name):
+    """fp16: one query head of two sees `n` keys. Returns q [1, 2, d], k and
+    v [n, 1, d], the outputs and how far each kernel's may be off them: a
+    weight is held to a step of 2^-24 after it was lifted by `lift`."""
+    d, n, down, how = FAINT[name]
+    log2 = 0.6931471805599453
+    q = torch.zeros(1, 2, d, dtype=torch.float16)
+    q[0, :, 0] = 1
+    gen = torch.Generator().manual_seed(n)
+    k = torch.zeros(n, 1, d, dtype=torch.float16)
+    v = (30000 + 30000 * torch.rand(n, 1, d, generator=gen)).half()
+    k[:, 0, 0] = -down * log2
+    top = {"first": [(0, 0.0)], "last": [(n - 1, 0.0)],
+           "rising": [(0, -5.5), (n // 3, -2.75), (n - 1, 0.0)]}[how]
+    for at, value in top:
+        k[at, 0, 0] = value * log2
+        v[at] = 0
+    w = torch.softmax(k[:, 0, 0].double(), 0)
+    out = (w @ v[:, 0].double())[None, None].expand(1, 2, d)
+
+    def tol(lift):
+        u = oracle.HALF_STEP[torch.float16]
+        off = u + 2 * (d + 32) * F32 * down + (n + 16) * F32
+        return u * out.abs() + off * out.abs() \
+            + 2.0 ** (-25 - lift) * v[:, 0].double().sum(0)
+
+    return q, k, v, out, tol

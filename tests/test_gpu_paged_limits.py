@@ -54,3 +54,21 @@ def test_packed_wild_values(name):
     args, kw, want = limits.packed_wild(name)
     out = ops.flash_prefill_packed_op(*(x.cuda() for x in args), **_cuda(kw))
     oracle.check("out", out, want["out"])
+
+
+@pytest.mark.parametrize("name", limits.FAINT)
+def test_faint_weights_in_fp16(name):
+    """Weights that 16 bits do not hold as they are."""
+    q, k, v, out, tol = limits.faint(name)
+    n, pages = len(k), -(-len(k) // 16)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    got = ops.flash_prefill_packed_op(q.cuda(), k.cuda(), v.cuda(), cu,
+                                      cu_seqlens_k=cu * n, scale=1.0)
+    oracle.check("prefill", got, (out, tol(9)))
+    pool = torch.zeros(2, pages * 16, 1, k.shape[2], dtype=k.dtype)
+    pool[0, :n], pool[1, :n] = k, v
+    pool = pool.view(2, pages, 16, 1, -1).cuda()
+    got = ops.paged_decode_op(
+        q.cuda(), pool[0], pool[1], torch.arange(pages, device="cuda")[None],
+        torch.tensor([n], device="cuda"), scale=1.0)
+    oracle.check("decode", got, (out, tol(15)))

@@ -47,6 +47,15 @@ template <int D> constexpr int kWavesOf = D == 64 ? 4 : 8;
 // A maximum may fall behind by this many powers of two before the sums are
 // rescaled: weights up to 2^6 cost no precision.
 constexpr float kSlack = 6.f;
+// Weights meet V in the inputs' type, the sum taken of them as they are before
+// that rounding: of bf16 2^-8 of each at most, which adds a quarter to an
+// output's error against 64 bits (packed prompts with a cap: 0.0017 to 0.0021),
+// where a second product for the rest would add half to the matrix work. fp16
+// has no numbers below 2^-24, so its weights are lifted by as much as the
+// slack leaves room for: they keep all bits down to 2^-23 of the maximum and
+// vanish below 2^-34 (2^-14 and 2^-25 without).
+template <typename T> constexpr float kLift = 0.f;
+template <> constexpr float kLift<_Float16> = 9.f;
 // Below this, in units of log2, a maximum is rounded by 2^-4 at most, which
 // scales a row's weights and their sum alike; logits past it are rounded like
 // the maximum before it is taken off. To keep both forms costs 8192 tokens
@@ -385,12 +394,12 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 2) void k_packed_prefill(
         far = far_off | __ballot(m != -INFINITY && fabsf(m) > kFar);
     }
     const float safe = m == -INFINITY ? 0.f : m;
-    from = add - safe;
+    from = add - safe + kLift<T>;
     if (far) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         s[r] = BIAS ? (s[r] + add) - safe : (s[r] * cf - safe) / cf;
-      from = 0.f;
+      from = kLift<T>;
     }
   };
   // 32 keys' scores in `s` are weighed and their values collected while the
@@ -531,7 +540,8 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 2) void k_packed_prefill(
   if (!live) return;
   if (a.lse && h == 0 && row0 + c < doc.m)
     a.lse[(long)(doc.q0 + row) * a.qh + head] =
-        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+        l == 0.f ? -INFINITY
+                 : (m - kLift<T> + __builtin_amdgcn_logf(l)) * kLn2;
   // Through LDS, where nothing is read any more, so that whole rows go out.
   constexpr int kRowO = D + 8;
   static_assert(kWaves * kRows * kRowO <= 2 * (kStageK + kStageV),

@@ -76,10 +76,14 @@ __global__ __launch_bounds__(256) void k_paged_append(
 //
 // The weights meet V in the inputs' type, as a rounded part and the rounded
 // rest: the second product is far from bounding the kernel, and with it the
-// output's own rounding is the only one that counts.
+// output's own rounding is the only one that counts. fp16 has no numbers
+// below 2^-24, so its weights are lifted by 2^15 while they are summed: of
+// those less than 2^-39 of the maximum nothing is left (2^-24 without).
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+template <typename T> constexpr float kLift = 1.f;
+template <> constexpr float kLift<_Float16> = 32768.f;
 constexpr int kTile = 32;              // keys of a wave's step
 constexpr int kStep = 4 * kTile;       // keys that chunks are measured in
 constexpr int kSlots = 512;            // workgroups that the card holds
@@ -438,7 +442,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = power_of(s[t][i], safe);
+        const float p = power_of(s[t][i], safe) * kLift<T>;
         l += p;
         hi[4 * t + i] = (T)p;
         lo[4 * t + i] = (T)(p - (float)hi[4 * t + i]);
@@ -491,6 +495,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
         if (acc[t][i] != acc[t][i] && alone[t][i] != 0.f)
           acc[t][i] = alone[t][i];
   }
+  l *= 1.f / kLift<T>;
+#pragma unroll
+  for (int t = 0; t < kT; ++t) acc[t] *= 1.f / kLift<T>;
   if (!cut.shared) {
     if (n >= heads) return;
     const float r = l == 0.f ? 0.f : 1.f / l;
