@@ -72,3 +72,50 @@ def test_faint_weights_in_fp16(name):
         q.cuda(), pool[0], pool[1], torch.arange(pages, device="cuda")[None],
         torch.tensor([n], device="cuda"), scale=1.0)
     oracle.check("decode", got, (out, tol(15)))
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_replays_past_the_table(weights):
+    """Steps that the host does not see: what has no slot is dropped, and
+    told; the rest is what eager steps leave. Then the host looks again."""
+    from triton_dist_amd.models import PagedKVCache
+
+    cache = PagedKVCache(1, 2, 32, 1, 64, block=16, device="cuda",
+                         weights=weights)
+    cache.reserve(16)
+    cache.begin_step(torch.tensor([13, 2], device="cuda"))
+    cu = torch.tensor([0, 13, 15], device="cuda")
+    x = torch.ones(15, 1, 64, device="cuda").bfloat16()
+    cache.write(0, x, x, cu)
+    cache.end_step()
+    x = torch.ones(2, 1, 64, device="cuda").bfloat16()
+
+    def step():
+        cache.begin_step()
+        cache.write(0, x, x)
+        out = cache.attend(0, x)
+        cache.end_step()
+        return out
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(20):
+        graph.replay()
+        torch.cuda.synchronize()
+        n = [14 + turn + 1, 3 + turn + 1]
+        assert cache.lost().tolist() == [m > 16 for m in n]
+        assert cache.seq_len.tolist() == [min(m, 32) for m in n]
+        assert (out == 1).all()
+    with pytest.raises(RuntimeError, match="no room"):
+        step()
+    cache.reserve(32)
+    assert cache.lost().tolist() == [True, True]
+    cache.reset()
+    cache.reserve(32)
+    for _ in range(32):
+        step()
+    with pytest.raises(RuntimeError, match="no room"):
+        step()
+    assert not cache.lost().any()

@@ -64,7 +64,12 @@ class PagedKVCache:
     and `attend`, then `end_step`, all of it without the host and for
     sequences of unlike lengths, so that a step can be captured. With
     `weights` the cache also keeps the attention weight that each slot got
-    and each slot's position, and `evict` cuts it to a budget by them."""
+    and each slot's position, and `evict` cuts it to a budget by them.
+
+    A step that the pages have no room for is refused by `begin_step`, where
+    the host knows of it. Where it does not, in a replayed graph or with
+    counts on the device, rows without a slot are dropped and `lost` tells
+    of them."""
 
     def __init__(self, n_layers: int, batch: int, max_len: int,
                  n_kv_heads: int, head_dim: int, block: int = 64,
@@ -90,6 +95,13 @@ class PagedKVCache:
         # of the step under way: its tokens, and the lengths with them
         self._count = torch.ones_like(self.seq_len)
         self._live = torch.zeros_like(self.seq_len)
+        # slots that every sequence has pages for, and what no length is
+        # above (None: not known), as far as the host was told; a captured
+        # step moves lengths whenever it is replayed
+        self._room, self._most, self._captured = 0, 0, False
+        # the longest that a sequence was to become, and which lost rows
+        self._peak = torch.zeros_like(self.seq_len)
+        self._lost = torch.zeros_like(self.seq_len, dtype=torch.bool)
         # the position of a sequence's next token, which eviction leaves
         self.next_pos = torch.zeros_like(self.seq_len)
         self.mass = self.key_pos = None
@@ -104,6 +116,9 @@ class PagedKVCache:
         self.seq_len.zero_()
         self.next_pos.zero_()
         self._free_top = 0
+        self._room, self._most = 0, 0
+        self._peak.zero_()
+        self._lost.zero_()
         if self.mass is not None:
             self.mass.zero_()
             self.key_pos.fill_(-1)
@@ -114,11 +129,52 @@ class PagedKVCache:
         host: once, outside of a captured step)."""
         if upto_len > self.max_len:
             raise ValueError(f"reserve: {upto_len} of {self.max_len} slots")
+        self._lost.logical_or_(self.lost())  # before there are more pages
         self._ensure_blocks(upto_len)
+
+    def _slots(self) -> torch.Tensor:
+        """[B]: slots from a sequence's first on whose pages are there."""
+        there = (self.block_table >= 0) & (self.block_table < self.n_blocks)
+        return there.long().cumprod(1).sum(1) * self.block
+
+    def lost(self) -> torch.Tensor:
+        """[B] bool: sequences that steps since the last `reset` wanted more
+        slots for than there are pages now, or were at a `reserve` since; rows
+        of theirs were dropped."""
+        return self._lost | (self._peak > self._slots())
+
+    def _make_sure(self, counts):
+        """Refuses a step that has no room. What the host was told decides;
+        if that does not, lengths and pages are looked at."""
+        if self.seq_len.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._captured = True
+            return
+        if isinstance(counts, torch.Tensor):
+            if counts.is_cuda:
+                self._most = None
+                return
+            new = int(counts.max()) if counts.numel() else 0
+        else:
+            new = int(counts)
+        if self._captured or self._most is None \
+                or self._most + new > self._room:
+            lens, slots = self.seq_len.cpu(), self._slots().cpu()
+            short = (lens + counts > slots).nonzero()[:, 0].tolist()
+            if short:
+                i = short[0]
+                raise RuntimeError(
+                    f"PagedKVCache: no room for the step in sequences "
+                    f"{short}; {i} holds {int(lens[i])} tokens and has pages "
+                    f"for {int(slots[i])} of {self.max_len} slots")
+            self._room = int(slots.min()) if self.batch else 0
+            self._most = int(lens.max()) if self.batch else 0
+        self._most += new
 
     def begin_step(self, counts=1):
         """A step that adds `counts` tokens to the sequences: one number, or
-        [B] of them."""
+        [B] of them. Raises RuntimeError, and changes nothing, if a sequence
+        has no pages for them; counts on the device are not looked at."""
+        self._make_sure(counts)
         if isinstance(counts, torch.Tensor):
             self._count.copy_(counts)
         else:
@@ -160,12 +216,15 @@ class PagedKVCache:
                                mass_out=self.mass[layer], **score)[0]
 
     def end_step(self):
-        self.seq_len.copy_(self._live)
+        torch.clamp(self._live, max=self.max_len, out=self.seq_len)
+        torch.maximum(self._peak, self._live, out=self._peak)
         self.next_pos.add_(self._count)
 
     def evict(self, budget: int, recent: int):
         """Between steps: cut every sequence to `budget` slots, in every
-        layer and for every key head by its own weights (`kv_evict_op`)."""
+        layer and for every key head by its own weights (`kv_evict_op`). A
+        next step needs a slot: the budget is to lie below what is reserved.
+        """
         from ..ops.paged import kv_evict_op
 
         if self.mass is None:
@@ -177,6 +236,8 @@ class PagedKVCache:
                         out=(self._live, self.mass[layer],
                              self.key_pos[layer]))
         self.seq_len.copy_(self._live)
+        if self._most is not None:
+            self._most = min(self._most, budget)
 
     def _ensure_blocks(self, upto_len: int):
         """Allocate pool blocks for every sequence up to `upto_len`
@@ -194,6 +255,7 @@ class PagedKVCache:
                                    device=table.device)
                 table[missing, j] = ids
                 self._free_top += n
+        self._room = max(self._room, need * self.block)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor,
                pos0: int):
@@ -210,6 +272,7 @@ class PagedKVCache:
             self.v_pool[layer, blk, p % self.block] = v[:, off]
         if layer == self.n_layers - 1:
             self.seq_len.fill_(pos0 + s)
+            self._most = pos0 + s
 
     def gather_layer(self, layer: int, upto_len: int):
         """Contiguous [B, upto_len, kvh, D] views for the decode kernels."""
