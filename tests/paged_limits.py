@@ -313,3 +313,75 @@ def faint(name):
             + 2.0 ** (-25 - lift) * v[:, 0].double().sum(0)
 
     return q, k, v, out, tol
+
+
+# block, budget, recent, pages that are not there, and what is kept of 100
+EVICT_GONE = {
+    "few": (16, 40, 4, [1, 5]), "first": (8, 90, 10, [0]),
+    "recent_gone": (16, 30, 20, [5, 6]), "most": (4, 40, 8, range(0, 25, 2)),
+    "more_than_budget": (4, 80, 8, [0, 3, 7, 9, 12, 20, 24]),
+    "nearly_all": (8, 20, 4, range(1, 13)), "all": (8, 20, 4, range(13)),
+    "block_one": (1, 37, 9, range(0, 100, 3)),
+}
+
+
+def evict_gone(name, n=100, heads=2):
+    """A sequence some of whose pages are not there, and the slots that
+    stay: present ones by age and weight, then the others by number."""
+    block, budget, recent, gone = EVICT_GONE[name]
+    gen = torch.Generator().manual_seed(len(name))
+    pages = -(-n // block)
+    table = torch.randperm(pages, generator=gen)[None].clone()
+    for p in gone:
+        table[0, p] = -1 if p % 2 else pages + 5
+    room = pages * block
+    k = torch.randn(pages, block, heads, 64, generator=gen).bfloat16()
+    v = torch.randn(pages, block, heads, 64, generator=gen).bfloat16()
+    mass = torch.rand(1, heads, room, generator=gen)
+    mass[..., ::9] = float("nan")
+    pos = torch.randperm(room, generator=gen).int().repeat(1, heads, 1)
+    there = [0 <= int(table[0, s // block]) < pages for s in range(n)]
+    kept = []
+    for h in range(heads):
+        newest = int(pos[0, h, :n].max())
+
+        def rank(s):
+            m = float(mass[0, h, s])
+            if not there[s]:
+                return 3, 0, s
+            if int(pos[0, h, s]) > newest - recent:
+                return 0, 0, s
+            return (1, 0, s) if m != m else (2, -m, s)
+        kept.append(sorted(sorted(range(n), key=rank)[:budget]))
+    return (k, v, table, torch.tensor([n])), mass, pos, budget, recent, \
+        there, kept
+
+
+def hold_evicted(before, after, mass, pos, got, budget, there, kept):
+    """Every slot that has a row now holds a kept row, its weight and its
+    position, and no kept row that a present slot is named for is another's."""
+    k, v, table, _ = before
+    gk, gv = after
+    lens, new_mass, new_pos = (x.cpu() for x in got)
+    assert lens.tolist() == [budget]
+    block = k.shape[1]
+
+    def row(pool, h, s):
+        return pool[table[0, s // block], s % block, h]
+
+    for h, slots in enumerate(kept):
+        stay = [s for s in slots if s < budget]
+        holes = [s for s in range(budget) if s not in slots]
+        movers = [s for s in slots if s >= budget]
+        of = dict(zip(stay + holes, stay + movers))
+        for s in range(budget):
+            at = of[s]
+            assert int(new_pos[0, h, s]) == int(pos[0, h, at])
+            x, y = float(new_mass[0, h, s]), float(mass[0, h, at])
+            assert x == y or x != x and y != y
+            if there[s]:  # then what it holds is the row it is named for
+                assert there[at]
+                assert torch.equal(row(gk.cpu(), h, s), row(k, h, at))
+                assert torch.equal(row(gv.cpu(), h, s), row(v, h, at))
+        assert (new_mass[0, h, budget:] == 0).all()
+        assert (new_pos[0, h, budget:] == -1).all()

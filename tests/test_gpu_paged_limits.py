@@ -119,3 +119,20 @@ def test_replays_past_the_table(weights):
     with pytest.raises(RuntimeError, match="no room"):
         step()
     assert not cache.lost().any()
+
+
+@pytest.mark.parametrize("name", limits.EVICT_GONE)
+@pytest.mark.parametrize("n, spare", [(100, 0), (100, 5000), (100, 20000)])
+def test_evict_where_pages_are_gone(name, n, spare):
+    """In each of the selection's forms, which go by the table's width."""
+    before, mass, pos, budget, recent, there, kept = limits.evict_gone(name,
+                                                                       n)
+    k, v, table, lens = (x.cuda() for x in before)
+    room = mass.shape[2] + -(-spare // k.shape[1]) * k.shape[1]
+    wide = torch.full((1, room // k.shape[1]), -1, device="cuda")
+    wide[:, :table.shape[1]] = table
+    more = torch.zeros(1, mass.shape[1], room - mass.shape[2], device="cuda")
+    got = ops.kv_evict_op(
+        k, v, wide, lens, torch.cat([mass.cuda(), more], 2),
+        torch.cat([pos.cuda(), more.int()], 2), budget, recent)
+    limits.hold_evicted(before, (k, v), mass, pos, got, budget, there, kept)

@@ -36,3 +36,26 @@ def test_packed_wild_values(name):
     args, kw, want = limits.packed_wild(name)
     oracle.check("out", ops.flash_prefill_packed_op(*args, **kw),
                  want["out"])
+
+
+@pytest.mark.parametrize("name", limits.EVICT_GONE)
+def test_evict_where_pages_are_gone(name):
+    before, mass, pos, budget, recent, there, kept = limits.evict_gone(name)
+    k, v, table, lens = (x.clone() for x in before)
+    got = ops.kv_evict_op(k, v, table, lens, mass, pos, budget, recent)
+    limits.hold_evicted(before, (k, v), mass, pos, got, budget, there, kept)
+
+
+def test_decode_after_a_cut_where_a_page_is_gone():
+    """An evicted row is not attended to under the name of one that was
+    never there."""
+    k = torch.zeros(2, 1, 1, 64).bfloat16()
+    v = torch.zeros_like(k)
+    v[0], v[1] = 5, 7
+    table, lens = torch.tensor([[0, 1, -1]]), torch.tensor([3])
+    mass, pos = torch.tensor([[[0.0, 5.0, 9.0]]]), torch.arange(3).int()
+    pos = pos.view(1, 1, 3)
+    lens, mass, pos = ops.kv_evict_op(k, v, table, lens, mass, pos, 1, 0)
+    assert pos.tolist() == [[[1, -1, -1]]]
+    q = torch.zeros(1, 1, 64).bfloat16()
+    assert (ops.paged_decode_op(q, k, v, table, lens) == 7).all()

@@ -682,7 +682,10 @@ __global__ __launch_bounds__(64 * kSpanWaves) void k_decode_finish(PagedDecodeAr
 // budget are not touched, so the steady state, one row over, moves one.
 // ---------------------------------------------------------------------------
 // Order of what stays: slots of the `recent` newest positions first, then
-// by weight, NaN above all as a sort has it. Unsigned compare; never 0.
+// by weight, NaN above all as a sort has it. Unsigned compare. 0 is no slot,
+// and kGone one whose page is not there: it holds no row that could move, so
+// it comes behind all others.
+constexpr unsigned kGone = 1;
 TD_DEV unsigned rank_key(float mass, bool is_recent) {
   if (is_recent) return 0xFFFFFFFFu;
   if (mass != mass) return 0xFFFFFFFEu;
@@ -707,7 +710,7 @@ struct Pair {
 template <int R, bool MANY>
 __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
                                                          int pairs) {
-  __shared__ int lds_n[kEvictWaves], hists[4][256];
+  __shared__ int lds_n[kEvictWaves], lds_gone[kEvictWaves], hists[4][256];
   __shared__ int lds_c[2][R][kEvictWaves], lds_all[2];
   const int b = blockIdx.x / a.c.kvh, h = blockIdx.x % a.c.kvh;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -737,6 +740,7 @@ __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
   float m[R];
   int p[R];
   long since = 0;
+  bool gone = false;  // some page of the sequence's is not there
   constexpr int kPart = R * kEvict;
   auto read = [&](int part) {
 #pragma unroll
@@ -753,19 +757,36 @@ __global__ __launch_bounds__(kEvict) void k_evict_select(EvictArgs a,
 #pragma unroll
       for (int r = 0; r < R; ++r) newest = max(newest, p[r]);
     }
+    const int used = (len - 1) / a.c.block + 1;
+    for (int i = tid; i < used; i += kEvict) {
+      const long page = a.c.table[b * a.c.table_stride + i];
+      gone |= page < 0 || page >= a.c.n_blocks;
+    }
     newest = wave_max(newest);
-    if (lane == 0) lds_n[wave] = newest;
+    gone = __any(gone);
+    if (lane == 0) lds_n[wave] = newest, lds_gone[wave] = gone;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kEvictWaves; ++i) newest = max(newest, lds_n[i]);
+    for (int i = 0; i < kEvictWaves; ++i) {
+      newest = max(newest, lds_n[i]);
+      gone |= lds_gone[i] != 0;
+    }
     since = (long)newest - a.recent + 1;
   }
   auto load = [&](int part) {
     if (MANY) read(part);
+    unsigned lacks = 0;  // bit r: a slot without a page
+    if (gone)
+#pragma unroll 1
+      for (int r = 0; r < R; ++r) {
+        const int i = part + r * kEvict + tid;
+        if (i < len && a.c.page(b, i) < 0) lacks |= 1u << r;
+      }
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      key[r] = part + r * kEvict + tid < len ? rank_key(m[r], p[r] >= since)
-                                             : 0;
+      key[r] = part + r * kEvict + tid >= len ? 0
+               : lacks >> r & 1               ? kGone
+                                              : rank_key(m[r], p[r] >= since);
   };
   if (!MANY) load(0);
 

@@ -393,7 +393,9 @@ def kv_evict_op(k_pool: torch.Tensor, v_pool: torch.Tensor,
     """Cut every sequence longer than `budget` slots to `budget`, per key
     head: the slots of the `recent` newest positions stay, and of the others
     those of the largest weight `mass` [B, kvh, room] fp32 (a NaN counts as
-    the largest, of equal ones the lowest slot stays).
+    the largest, of equal ones the lowest slot stays). A slot whose page is
+    not there holds no row: it stays only if all that have one do, the lowest
+    first.
 
     The rows that stay are moved into the slots below the budget in place:
     the i-th slot below it that became free takes the i-th kept row from
@@ -403,7 +405,8 @@ def kv_evict_op(k_pool: torch.Tensor, v_pool: torch.Tensor,
 
     Returns the lengths, weights and positions afterwards, with 0 and -1 in
     the slots past the new length: new tensors, or those of `out`, which may
-    be the inputs themselves. A page is moved by the one sequence that holds
+    be the inputs themselves. A row that would move to a page that is not
+    there is dropped. A page is moved by the one sequence that holds
     it: pages that sequences share must not be evicted from.
     """
     fields, (block, kvh, d, b, room) = _cache(k_pool, v_pool, block_table,
@@ -450,12 +453,15 @@ def kv_evict_op(k_pool: torch.Tensor, v_pool: torch.Tensor,
     for i in range(b):
         length = min(max(int(seq_lens[i]), 0), room)
         keep = min(length, budget)
+        page = block_table[i].long()[torch.arange(length) // block]
+        there = (page >= 0) & (page < n)
         for h in range(kvh if length > keep else 0):
             m, p = mass[i, h, :length], key_pos[i, h, :length].long()
             fresh = p > int(p.max()) - recent
             order = torch.sort(m, descending=True, stable=True).indices
-            order = torch.cat([torch.nonzero(fresh)[:, 0],
-                               order[~fresh[order]]])
+            order = torch.cat([torch.nonzero(fresh & there)[:, 0],
+                               order[(~fresh & there)[order]],
+                               torch.nonzero(~there)[:, 0]])
             kept = torch.zeros(length, dtype=torch.bool)
             kept[order[:keep]] = True
             holes = torch.nonzero(~kept[:keep])[:, 0].tolist()
