@@ -59,3 +59,37 @@ def test_decode_after_a_cut_where_a_page_is_gone():
     assert pos.tolist() == [[[1, -1, -1]]]
     q = torch.zeros(1, 1, 64).bfloat16()
     assert (ops.paged_decode_op(q, k, v, table, lens) == 7).all()
+
+
+def _cache_fields(b=1, block=64, kvh=8, width=8):
+    """A cache as the native functions take it, at no address."""
+    return [0, 0, block * kvh * 64, kvh * 64, 64, block * kvh * 64, kvh * 64,
+            64, 1, block, kvh, 64, 0, 0, 0, width, width, 0, 1, b]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(),
+                    reason="what is not refused would run")
+@pytest.mark.parametrize("name, args", [
+    ("paged_append", (_cache_fields(), 0, 0, 0, 0, 0, 0, 1 << 27, 0, 0, 0, 0,
+                      0, 0)),
+    ("paged_decode", (_cache_fields(b=1 << 24), 0, 0, 0, 8, 1.0, 0.0, 0, 0,
+                      0, 0, 0, 0, 0, 0, 0, 0)),
+    # as many slots as there may be without weights, and one of 65535 less
+    # than the joins and the spans of 1024 slots need with them
+    ("paged_decode", (_cache_fields(kvh=1, width=(65535 - 31) * 16), 0, 0, 0,
+                      32, 1.0, 0.0, 0, 0, 0, 0, 0, 0, 1, 1, 0, 0)),
+    ("paged_decode", (_cache_fields(kvh=1 << 16), 0, 0, 0, 1 << 16, 1.0, 0.0,
+                      0, 0, 0, 0, 0, 0, 0, 0, 0, 0)),
+    ("kv_evict", (_cache_fields(b=1 << 22), 0, 0, 5, 1, 0, 0, 0, 0, 0)),
+    ("kv_evict", (_cache_fields(width=1 << 17), 0, 0, 1 << 22, 1, 0, 0, 0, 0,
+                  0)),
+    ("packed_prefill", (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1 << 30, 1,
+                        64, 8, 128, 0, 1, 0, 0, 0, 0, 0, 0, 1, 1, 1.0, 0.0,
+                        0, 0)),
+])
+def test_too_large_for_a_launch(name, args):
+    """Refused before anything is launched."""
+    from triton_dist_amd import _C
+
+    with pytest.raises(RuntimeError, match="too (large|many)"):
+        getattr(_C, name)(*args)

@@ -576,7 +576,7 @@ void prefill(const PackedArgs &a, hipStream_t stream) {
   constexpr int kWaves = kWavesOf<D>;
   const long g = a.qh / a.kvh;
   const long tiles = (a.rows / kRows + a.seqs) * g / kWaves + a.seqs + 4;
-  if (tiles * a.kvh > 0x7fffffffL)
+  if (tiles * a.kvh * 64 * kWaves > 0xffffffffL)  // threads of a launch
     throw std::runtime_error("packed_prefill: too many rows and heads");
   const dim3 grid((unsigned)(tiles * a.kvh));
   const int n = 64 * kWaves, t = (int)tiles;

@@ -19,6 +19,16 @@ void launched(const char *what) {
     throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
 }
 
+// A launch counts threads in 32 bits, and workgroups past the first dimension
+// in 16.
+void check_grid(const char *what, long x, long threads, long y = 1,
+                long z = 1) {
+  if (x * threads > 0xffffffffL || y > 0xffff || z > 0xffff)
+    throw std::runtime_error(
+        std::string(what) + ": too large, " + std::to_string(x) + " x " +
+        std::to_string(y) + " x " + std::to_string(z) + " workgroups");
+}
+
 // ---------------------------------------------------------------------------
 // append: one thread moves 16 bytes of a token's keys and values.
 // ---------------------------------------------------------------------------
@@ -973,8 +983,7 @@ void launch_paged_append(const PagedArgs &a, const void *k, long k_tok,
                          hipStream_t stream) {
   const long threads = tokens * a.kvh * (a.d / 8);
   if (!threads || !a.batch) return;
-  if (threads > 0x7fffffffL * 256)
-    throw std::runtime_error("paged_append: too many tokens");
+  check_grid("paged_append", (threads + 255) / 256, 256);
   k_paged_append<<<dim3((unsigned)((threads + 255) / 256)), 256, 0, stream>>>(
       a, (const bf16 *)k, k_tok, k_head, (const bf16 *)v, v_tok, v_head,
       tokens, cu, key_pos, pos);
@@ -1016,13 +1025,16 @@ static void decode(const PagedDecodeArgs &a, const DecodeWork &w,
   const long shared = a.c.batch + (kSlots + per - 1) / per;
   const long apart = a.c.batch + (2 * kSlots + own - 1) / own;
   const long blocks = max(w.apart ? 0 : shared * per, apart * own);
-  if (blocks > 0x7fffffffL)
-    throw std::runtime_error("paged_decode: too many sequences and heads");
+  // nothing to join where no sequence can have two chunks
+  const long spans = a.mass ? (a.c.room() + kSpan - 1L) / kSpan : 0;
+  const bool more = spans || a.c.room() > w.least * kStep;
+  check_grid("paged_decode", blocks, 256);
+  if (more)
+    check_grid("paged_decode", a.c.batch, 64 * kSpanWaves, a.c.kvh,
+               w.joins + spans);
   k_paged_decode<T, D><<<dim3((unsigned)blocks), 256, 0, stream>>>(a, w);
   launched("paged_decode");
-  // nothing to join where no sequence can have two chunks
-  const int spans = a.mass ? (a.c.room() + kSpan - 1) / kSpan : 0;
-  if (spans || a.c.room() > w.least * kStep) {
+  if (more) {
     const dim3 finish(a.c.batch, a.c.kvh, w.joins + spans);
     k_decode_finish<T, D><<<finish, 64 * kSpanWaves, 0, stream>>>(a, w);
     launched("paged_decode");
@@ -1031,9 +1043,6 @@ static void decode(const PagedDecodeArgs &a, const DecodeWork &w,
 
 void launch_paged_decode(const PagedDecodeArgs &a, hipStream_t stream) {
   if (!a.c.batch) return;
-  if (a.c.kvh > 65535 || a.c.room() / kSpan > 65000)
-    throw std::runtime_error("paged_decode: 65535 key heads and 2^25 slots of "
-                             "a sequence at most");
   if ((long)a.c.batch * (a.c.room() / kStep + 1) > 1L << 30)
     throw std::runtime_error("paged_decode: 2^37 slots in all at most");
   DecodeWork w = decode_work(a.c.batch, a.qh, a.c.kvh);
@@ -1065,8 +1074,10 @@ void launch_kv_evict(const EvictArgs &a, hipStream_t stream) {
   const int room = a.c.room(), pairs = evict_pairs(room, a.budget);
   const long rows = (long)a.c.batch * a.c.kvh;
   const long parts = (pairs + kPairs - 1) / kPairs;
-  if (rows > 0x7fffffffL || parts > 65535 || room > 1 << 30)
-    throw std::runtime_error("kv_evict: too many sequences, heads or slots");
+  if (room > 1 << 30)
+    throw std::runtime_error("kv_evict: 2^30 slots of a sequence at most");
+  check_grid("kv_evict", rows, kEvict);
+  check_grid("kv_evict", rows, 256, parts);
   // registers for as many keys as a sequence can have, in steps that each
   // cost the shorter ones something
   if (room <= 4 * kEvict)
