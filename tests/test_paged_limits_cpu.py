@@ -93,3 +93,98 @@ def test_too_large_for_a_launch(name, args):
 
     with pytest.raises(RuntimeError, match="too (large|many)"):
         getattr(_C, name)(*args)
+
+
+def _pools(kind, n=3, block=4, heads=2, d=16):
+    """Pools and whether rows of theirs share memory."""
+    store = torch.zeros(4 * n * block * heads * d).bfloat16()
+    shape, row = (n, block, heads, d), heads * d
+    whole = (block * row, row, d, 1)
+    if kind == "apart":
+        return torch.zeros(shape).bfloat16(), torch.zeros(shape).bfloat16()
+    if kind == "one":
+        k = store.as_strided(shape, whole)
+        return k, store.as_strided(shape, whole)
+    if kind == "heads_side_by_side":
+        kv = store[:2 * n * block * row].view(n, block, 2 * heads, d)
+        return kv[:, :, :heads], kv[:, :, heads:]
+    if kind == "heads_in_turn":
+        kv = store[:2 * n * block * row].view(n, block, heads, 2, d)
+        return kv[..., 0, :], kv[..., 1, :]
+    if kind == "pages_in_turn":
+        kv = store[:2 * n * block * row].view(n, 2, block, heads, d)
+        return kv[:, 1], kv[:, 0]
+    if kind == "head_major":
+        kv = store[:2 * n * block * row].view(2, n, heads, block, d)
+        return kv[0].transpose(1, 2), kv[1].transpose(1, 2)
+    if kind == "one_page_each":  # a stride that nothing steps by
+        return store[:block * row].view(1, block, heads, d).expand(
+            1, -1, -1, -1), torch.zeros(1, *shape[1:]).bfloat16()
+    k = store.as_strided(shape, whole)
+    return {
+        "a_page_on": lambda: (k, store.as_strided(shape, whole,
+                                                  block * row)),
+        "a_row_back": lambda: (store.as_strided(shape, whole, row), k),
+        "half_a_row_on": lambda: (k, store.as_strided(shape, whole, d // 2)),
+        "other_strides": lambda: (k, store.as_strided(
+            shape, (row, n * row, d, 1))),
+        "expanded_pages": lambda: (k[:1].expand(shape), k.clone()),
+        "expanded_heads": lambda: (k.clone(), k[:, :, :1].expand(shape)),
+        "folded_rows": lambda: (k.clone(), store.as_strided(
+            shape, (block * row, 8, d, 1))),
+    }[kind]()
+
+
+GOOD = ["apart", "one", "heads_side_by_side", "heads_in_turn",
+        "pages_in_turn", "head_major", "one_page_each"]
+SHARING = ["a_page_on", "a_row_back", "half_a_row_on", "other_strides",
+           "expanded_pages", "expanded_heads", "folded_rows"]
+
+
+@pytest.mark.parametrize("kind", GOOD + SHARING)
+def test_pools_that_share_memory(kind):
+    """Refused where they are written; reading them is fine."""
+    k_pool, v_pool = _pools(kind)
+    table, lens = torch.tensor([[0, 2], [1, -1]]), torch.tensor([5, 0])
+    if len(k_pool) == 1:
+        table = table.clamp(max=0)
+    k = torch.randn(2, 2, 16).bfloat16()
+    v = k if kind == "one" else torch.randn(2, 2, 16).bfloat16()
+    mass = torch.zeros(2, 2, 8)
+    calls = [lambda: ops.paged_append_op(k, v, k_pool, v_pool, table, lens),
+             lambda: ops.kv_evict_op(k_pool, v_pool, table, lens, mass,
+                                     mass.int(), 2, 1)]
+    for call in calls:
+        if kind in SHARING:
+            with pytest.raises(ValueError, match="pool: "):
+                call()
+        else:
+            call()
+    if kind in GOOD and kind != "one_page_each":
+        ops.paged_append_op(k, v, k_pool, v_pool, table, lens)
+        assert torch.equal(k_pool[2, 1], k[0])
+        assert torch.equal(v_pool[2, 1], v[0])
+        assert torch.equal(k_pool[1, 0], k[1])
+        assert torch.equal(v_pool[1, 0], v[1])
+
+
+def test_pools_in_decode_may_share_memory():
+    store = torch.randn(3 * 16 * 64).bfloat16()
+    pool = store.view(3, 16, 1, 64)
+    q = torch.randn(1, 2, 64).bfloat16()
+    table, lens = torch.tensor([[2, 1]]), torch.tensor([20])
+    want = ops.paged_decode_op(q, pool, pool.clone(), table, lens)
+    assert torch.equal(ops.paged_decode_op(q, pool, pool, table, lens), want)
+
+
+def test_append_refuses_rows_of_the_pools():
+    pool = torch.zeros(3, 4, 2, 16).bfloat16()
+    at = (pool, pool.clone(), torch.tensor([[0], [1]]), torch.tensor([0, 0]))
+    new = torch.randn(2, 2, 16).bfloat16()
+    for k, v in ((pool[2, :2], new), (new, pool[2, :2]),
+                 (at[1][2, :2], new), (pool[1:, 0], new)):
+        with pytest.raises(ValueError, match="apart from the pools"):
+            ops.paged_append_op(k, v, *at)
+    ops.paged_append_op(pool[2, :2].clone(), new, *at)
+    with pytest.raises(ValueError, match="one k as v"):
+        ops.paged_append_op(new, new.clone(), pool, pool, *at[2:])

@@ -147,6 +147,48 @@ def _cache(k_pool, v_pool, block_table, seq_lens):
         (block, kvh, d, b, width * block)
 
 
+def _meet(apart: int, dims, d: int) -> bool:
+    """Whether rows of d elements of two tensors of the same strides `dims`
+    (from the largest, with sizes), whose first elements lie `apart`, have an
+    element in common."""
+    if not dims:
+        return abs(apart) < d
+    (stride, size), rest = dims[0], dims[1:]
+    if stride == 0 or size == 1:
+        return _meet(apart, rest, d)
+    near = apart // stride
+    return any(_meet(apart - i * stride, rest, d) for i in (near, near + 1)
+               if abs(i) < size)
+
+
+def _writes(k_pool, v_pool, fields):
+    """Pools that a call writes: rows have memory of their own, also in the
+    other pool unless both are one. Returns where each begins and ends."""
+    k, v, k0, k1, k2, v0, v1, v2, n, block, kvh, d = fields[:12]
+    if k_pool.is_contiguous() and v_pool.is_contiguous():
+        size = 2 * n * block * kvh * d
+        k_end, v_end = k + size, v + size
+        if k_end <= v or v_end <= k or k == v:
+            return k, k_end, v, v_end
+    else:
+        for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
+            reach = d
+            for stride, size in sorted(zip(t.stride(), t.shape[:3])):
+                if size > 1:
+                    if stride < reach:
+                        _refuse(f"{name}: rows that do not share memory")
+                    reach += stride * (size - 1)
+        k_end = k + 2 * ((n - 1) * k0 + (block - 1) * k1 + (kvh - 1) * k2 + d)
+        v_end = v + 2 * ((n - 1) * v0 + (block - 1) * v1 + (kvh - 1) * v2 + d)
+    if k < v_end and v < k_end:
+        same = (k0, k1, k2) == (v0, v1, v2)
+        if not (same and k == v) and (not same or _meet(
+                (v - k) // 2, sorted(((k0, n), (k1, block), (k2, kvh)),
+                                     reverse=True), d)):
+            _refuse("v_pool: k_pool itself, or apart from it")
+    return k, k_end, v, v_end
+
+
 def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -197,6 +239,10 @@ def paged_append_op(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
     without room (past the table, or on a page that is not there) is
     dropped. `key_pos` [B, kvh, room] int32, if given, gets the tokens'
     positions `pos` [T] at their slots.
+
+    The pools' rows have memory of their own, apart from each other (one pool
+    may hold what serves as both) and from k and v. No two tokens may be for
+    the same row: sequences that share a page write behind it.
     """
     fields, (block, kvh, d, b, room) = _cache(k_pool, v_pool, block_table,
                                               seq_lens)
@@ -221,9 +267,19 @@ def paged_append_op(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
         _refuse("key_pos and pos: both or neither")
     if not tokens or not b:
         return
+    x, y = k.data_ptr(), v.data_ptr()
+    x0, x1, _ = k.stride()
+    y0, y1, _ = v.stride()
+    begin, end, begin2, end2 = _writes(k_pool, v_pool, fields)
+    x_end = x + 2 * ((tokens - 1) * x0 + (kvh - 1) * x1 + d)
+    y_end = y + 2 * ((tokens - 1) * y0 + (kvh - 1) * y1 + d)
+    if x < end and begin < x_end or x < end2 and begin2 < x_end \
+            or y < end and begin < y_end or y < end2 and begin2 < y_end:
+        _refuse("k and v: apart from the pools")
+    if begin == begin2 and (x, x0, x1) != (y, y0, y1):
+        _refuse("k_pool and v_pool: one pool takes one k as v")
     if dev.type == "cuda":
-        _call("paged_append", dev, fields, k.data_ptr(), k.stride(0),
-              k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), tokens,
+        _call("paged_append", dev, fields, x, x0, x1, y, y0, y1, tokens,
               _ptr(cu_seqlens), _is64(cu_seqlens), _ptr(key_pos), _ptr(pos),
               _is64(pos))
         return
@@ -412,6 +468,7 @@ def kv_evict_op(k_pool: torch.Tensor, v_pool: torch.Tensor,
     fields, (block, kvh, d, b, room) = _cache(k_pool, v_pool, block_table,
                                               seq_lens)
     dev = k_pool.device
+    _writes(k_pool, v_pool, fields)
     if mass.requires_grad and torch.is_grad_enabled():
         _no_backward()
     _array("mass", mass, _F32, (b, kvh, room), dev)
