@@ -188,3 +188,40 @@ def test_append_refuses_rows_of_the_pools():
     ops.paged_append_op(pool[2, :2].clone(), new, *at)
     with pytest.raises(ValueError, match="one k as v"):
         ops.paged_append_op(new, new.clone(), pool, pool, *at[2:])
+
+
+def test_forward_derivatives_are_refused():
+    """Each input that could carry one; the same calls go through without."""
+    import torch.autograd.forward_ad as forward
+
+    def call(name, change):
+        def f(key, shape, dtype=torch.bfloat16):
+            return change(key, torch.zeros(shape, dtype=dtype))
+        pools = f("k_pool", (2, 4, 1, 64)), f("v_pool", (2, 4, 1, 64))
+        at = torch.tensor([[0, 1]]), torch.tensor([6])
+        mass = f("mass", (1, 1, 8), torch.float32)
+        slopes = f("slopes", (1,), torch.float32)
+        q = f("q", (1, 1, 64))
+        if name == "append":
+            ops.paged_append_op(f("k", (1, 1, 64)), f("v", (1, 1, 64)),
+                                *pools, *at)
+        elif name == "decode":
+            ops.paged_decode_op(q, *pools, *at, mass=mass, slopes=slopes)
+        elif name == "evict":
+            ops.kv_evict_op(*pools, *at, mass,
+                            torch.zeros(1, 1, 8, dtype=torch.int32), 3, 1)
+        else:
+            ops.flash_prefill_packed_op(
+                q, f("k", (1, 1, 64)), f("v", (1, 1, 64)),
+                torch.tensor([0, 1]), slopes=slopes)
+
+    with forward.dual_level():
+        for name, keys in (("append", "k v k_pool v_pool"),
+                           ("decode", "q k_pool v_pool mass slopes"),
+                           ("evict", "k_pool v_pool mass"),
+                           ("prefill", "q k v slopes")):
+            call(name, lambda key, t: t)
+            for which in keys.split():
+                with pytest.raises(RuntimeError, match="forward derivative"):
+                    call(name, lambda key, t: forward.make_dual(
+                        t, torch.ones_like(t)) if key == which else t)

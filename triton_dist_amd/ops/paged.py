@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 _BF16, _FP16 = torch.bfloat16, torch.float16
@@ -55,6 +56,16 @@ def _refuse(message: str):
 def _no_backward():
     raise RuntimeError("this operator has no backward: call it under "
                        "torch.no_grad() or detach its inputs")
+
+
+def _no_tangents(*tensors):
+    """Forward-mode derivatives, which need no requires_grad, would vanish."""
+    if _forward._current_level < 0:
+        return
+    if any(t is not None and _forward.unpack_dual(t).tangent is not None
+           for t in tensors):
+        raise RuntimeError("this operator has no forward derivative: give it "
+                           "the primal of its inputs")
 
 
 def _rows16(name: str, t: torch.Tensor):
@@ -249,6 +260,7 @@ def paged_append_op(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
     dev, dtype = k_pool.device, k_pool.dtype
     if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         _no_backward()
+    _no_tangents(k, v, k_pool, v_pool)
     tokens = k.shape[0]
     if k.shape != (tokens, kvh, d) or v.shape != k.shape:
         _refuse(f"k: and v: [T, {kvh}, {d}], got {tuple(k.shape)} and "
@@ -341,6 +353,7 @@ def paged_decode_op(q: torch.Tensor, k_pool: torch.Tensor,
             q.requires_grad or mass is not None and mass.requires_grad
             or slopes is not None and slopes.requires_grad):
         _no_backward()
+    _no_tangents(q, k_pool, v_pool, mass, slopes)
     if q.dim() != 3 or q.shape[0] != b or q.shape[2] != d:
         _refuse(f"q: [{b}, qh, {d}], got {tuple(q.shape)}")
     qh = q.shape[1]
@@ -471,6 +484,7 @@ def kv_evict_op(k_pool: torch.Tensor, v_pool: torch.Tensor,
     _writes(k_pool, v_pool, fields)
     if mass.requires_grad and torch.is_grad_enabled():
         _no_backward()
+    _no_tangents(k_pool, v_pool, mass)
     _array("mass", mass, _F32, (b, kvh, room), dev)
     _array("key_pos", key_pos, _I32, (b, kvh, room), dev)
     budget, recent = int(budget), int(recent)
@@ -589,6 +603,7 @@ def flash_prefill_packed_op(q: torch.Tensor, k: torch.Tensor,
             q.requires_grad or k.requires_grad or v.requires_grad
             or slopes is not None and slopes.requires_grad):
         _no_backward()
+    _no_tangents(q, k, v, slopes, out)
     _heads("q", q, dtype, dev)
     _heads("k", k, dtype, dev)
     _heads("v", v, dtype, dev)
