@@ -40,9 +40,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kRows = 32, kKeys = 64;
 // Of a workgroup. With rows of 64 elements more of a step's work is vector
-// instructions, and two workgroups of four on a SIMD's waves overlap better
-// (16384 tokens, capped: 1.70 ms for 1.90); with 128 sharing K and V among
-// eight does (plain: 2.32 ms for 2.43).
+// instructions, and two workgroups of four on a SIMD's waves overlap better:
+// 8 heads, 8192 tokens plain 139 us for 156 with eight, capped 171 for 240,
+// 1000 tokens 22 for 25, 64 documents of 256 24 for 29, 8 of 1000 the same.
+// With 128 sharing K and V among eight does where documents are long: 8192
+// tokens, 32 query heads plain 569 us for 610 with four, capped 675 for 702.
+// Where they are short four would do better: 64 documents of 256 146 for 116,
+// one of 1000 35 for 30.
 template <int D> constexpr int kWavesOf = D == 64 ? 4 : 8;
 // A maximum may fall behind by this many powers of two before the sums are
 // rescaled: weights up to 2^6 cost no precision.
@@ -522,7 +526,15 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 2) void k_packed_prefill(
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) {
       f32x16 alone = {};
+#pragma unroll 4
       for (int key = 0; key < most; ++key) {
+        if (key % 64 == 0) {  // done where all that were NaN are by a value
+          bool open = false;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            open |= acc[t][r] != acc[t][r] && alone[r] == alone[r];
+          if (!__any(open && key < lim)) break;
+        }
         if (key >= lim) continue;
         const T *v = (const T *)a.v + (long)(doc.k0 + key) * a.v_tok +
                      kh * a.v_head + 4 * h + 32 * t;

@@ -97,7 +97,11 @@ template <> constexpr float kLift<_Float16> = 32768.f;
 constexpr int kTile = 32;              // keys of a wave's step
 constexpr int kStep = 4 * kTile;       // keys that chunks are measured in
 constexpr int kSlots = 512;            // workgroups that the card holds
-constexpr int kFew = 6;                // steps that a workgroup starts for
+// Steps that a workgroup starts for. Neither side of it suits all: at 12,
+// 16 sequences of 4000 keys with 8 key heads take 55 us for 61 and 100 of 500
+// 50 for 58, but 512 of 131 take 70 for 63; at 3, 64 of up to 4100 with 4 key
+// heads take 58 for 61, but one of 30000 with 8 takes 37 for 33.
+constexpr int kFew = 6;
 
 template <typename T> using vec8 = __attribute__((ext_vector_type(8))) T;
 template <typename T> using vec4 = __attribute__((ext_vector_type(4))) T;
@@ -483,7 +487,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
   if (__any(spoilt && l == l)) {
     f32x4 alone[kT] = {};
     for (base = k0 + (cut.shared ? wave * kTile : 0); base < k1;
-         base += stride)
+         base += stride) {
+      bool open = false;  // NaN, and not yet by a value
+#pragma unroll
+      for (int t = 0; t < kT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          open |= acc[t][i] != acc[t][i] && alone[t][i] == alone[t][i];
+      if (!__any(open)) break;
+#pragma unroll 4
       for (int slot = base; slot < min(base + kTile, k1); ++slot) {
         const long p = a.c.page(b, slot);
         if (p < 0) continue;
@@ -498,6 +510,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_decode(PagedDecodeArgs a,
             alone[t][i] += wild(x[i]) ? (float)x[i] : 0.f;
         }
       }
+    }
 #pragma unroll
     for (int t = 0; t < kT; ++t)
 #pragma unroll
@@ -995,6 +1008,9 @@ static DecodeWork decode_work(int batch, int qh, int kvh) {
   w.groups = (qh / kvh + 15) / 16;
   // so many sequences that there are steps enough, if none is empty
   w.apart = (long)batch * kvh * w.groups >= kFew * kSlots;
+  // ... and of these each then takes two at least, since a sequence of one to
+  // two steps in two chunks costs a join (512 of 131 keys, 8 key heads: 65 us
+  // for 63; 400 of 131 in rows of 64: 36 for 33; longer ones the same)
   w.least = w.apart ? 2 : 1;
   // a workgroup to a query head, unless so many would take longer to start
   // than to join (512 sequences, 8 key heads, nothing to join: 17 us)
