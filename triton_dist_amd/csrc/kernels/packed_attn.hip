@@ -374,7 +374,8 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 2) void k_packed_prefill(
   // is then the power of s * cf + from (s + from with a bias): one operation
   // a score, which takes the maximum off the unrounded product, so that the
   // largest weight is 2 to the rounding of the maximum. Where that could be
-  // far from 1, logits are rounded like the maximum before it is taken off.
+  // far from 1, logits are rounded like the maximum before it is taken off (and
+  // divided by the cf that the power multiplies them by).
   float from = 0.f;
   const unsigned long long far_off =
       BIAS ? __ballot(fabsf(slope) * (float)max(abs(pos), abs(pos - doc.n)) +
