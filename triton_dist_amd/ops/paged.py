@@ -344,7 +344,8 @@ def paged_decode_op(q: torch.Tensor, k_pool: torch.Tensor,
     Returns out [B, qh, d], and in this order, where asked for, the log of
     the sum of exponentials [B, qh] fp32 and the weights. A sequence that
     sees no key gets zeros and -inf. A value that is no finite number counts
-    in full, however small its weight is.
+    in full, however small its weight is. Values are summed in 32 bits before
+    the weights' sum divides them, so finite ones are to stay below 2^90.
     """
     fields, (block, kvh, d, b, room) = _cache(k_pool, v_pool, block_table,
                                               seq_lens)
@@ -582,7 +583,8 @@ def flash_prefill_packed_op(q: torch.Tensor, k: torch.Tensor,
     and are zeros and -inf in tensors that the call makes (a `lse` always).
     What the mask hides from a query does not count, whatever it holds; a
     value that is seen and is no finite number counts in full, however small
-    its weight is.
+    its weight is, and finite ones are to stay below 2^90, as in
+    `paged_decode_op`.
     """
     dev, dtype = q.device, q.dtype
     if q.dim() != 3 or k.dim() != 3:
